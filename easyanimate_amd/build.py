@@ -22,7 +22,9 @@ if _OUT:
     LIB = os.path.abspath(_OUT)
     LIBDIR = os.path.dirname(LIB)
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value"]
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 in the device code (the compiler forms them from ordinary float code; some of their forms
+# are not reliable on this chip).  The host pass does not know the feature and says so: harmless.
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # per-file extras: the one-wave-per-SIMD attention kernel keeps its MFMA accumulators in arch VGPRs (they are read by
 # the softmax VALU code every block); without this hipcc parks them in AGPRs and copies ~340 registers per tile.
 FLAGS += os.environ.get("EA_HIPCC_EXTRA", "").split()   # diagnostic builds, e.g. EA_HIPCC_EXTRA=-DEA_GEMM_TIMESTAMPS
