@@ -12,6 +12,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
 
+def pytest_collection_modifyitems(items):
+    # its deliberate out-of-range read is a GPU memory fault in a child process; a faulting kernel can take the whole card down
+    for it in items:
+        if it.nodeid.endswith("test_fence_gpu.py::test_fence_positive_control"):
+            it.add_marker(pytest.mark.skip(reason="faults the GPU on purpose; no test run may"))
+
+
 @pytest.fixture(scope="session")
 def lib_built():
     """Make sure libea_mi355x.so exists (hipcc cross-compiles without a GPU)."""
