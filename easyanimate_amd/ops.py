@@ -5,8 +5,9 @@ HIP kernel in libea_mi355x.so.  There is no CPU / eager fallback: CPU tensors ra
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
-from typing import Optional
+from typing import NamedTuple, Optional, Union
 
 import torch
 
@@ -239,6 +240,128 @@ def gemm_kblocked(A: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor]
     _timed("gemm", lambda: _lib.call("ea_gemm_bf16_kblocked", _p(A), _p(W), _p(bias), _p(out), _p(res), _p(gate), B, M, N, K, A.stride(0),
                                      out.stride(0), ldres, rbs, gbs, int(epilogue), int(layout), _stream()))
     return out
+
+
+# ---- microscaled 4-bit storage --------------------------------------------------------------------
+class Mxfp4(NamedTuple):
+    """A [rows, k] matrix in microscaled 4-bit storage (mxfp4_quantize): codes uint8 [ceil(k/256), rows, 128] (two e2m1 codes a byte,
+    low nibble first), scales uint8 [ceil(k/256), rows, 8] (2^(byte - 127) per block of 32 elements of a row; 255 = NaN)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    rows: int
+    k: int
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _same_device(dev: torch.device, *ts):
+    """All tensors on `dev` (a GPU); returns the context that makes it the current device, so that the launch goes to that device's
+    current stream whatever device the caller has selected."""
+    for t in ts:
+        if t is not None and t.device != dev:
+            _dev(t)
+            raise RuntimeError(f"easyanimate_amd.ops: tensors on different devices ({dev} and {t.device})")
+    if dev.type != "cuda":
+        raise RuntimeError("easyanimate_amd.ops: tensors must live on the GPU -- the hot path has no CPU fallback")
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _chk_mxfp4(t: Mxfp4, name: str):
+    kt = (t.k + 255) // 256
+    if t.codes.dtype != torch.uint8 or t.scales.dtype != torch.uint8:
+        raise TypeError(f"{name}: codes and scales must be uint8")
+    if t.k < 1 or t.codes.shape != (kt, t.rows, 128) or t.scales.shape != (kt, t.rows, 8):
+        raise ValueError(f"{name}: codes {tuple(t.codes.shape)} / scales {tuple(t.scales.shape)} are not those of a [{t.rows}, {t.k}] matrix")
+    if not (t.codes.is_contiguous() and t.scales.is_contiguous()):
+        raise ValueError(f"{name}: codes and scales must be contiguous")
+
+
+def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
+    """x bf16 [rows, k] (inner stride 1, row stride free) -> its microscaled 4-bit storage (ea_mxfp4_quantize_bf16)."""
+    _chk(x, _BF16, "x")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x: expected [rows, k >= 1], got {tuple(x.shape)}")
+    rows, k = x.shape
+    if rows > 1 and (x.stride(1) != 1 or x.stride(0) < k) or k > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    kt = (k + 255) // 256
+    with _same_device(x.device):
+        codes = torch.empty((kt, rows, 128), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((kt, rows, 8), dtype=torch.uint8, device=x.device)
+        _lib.call("ea_mxfp4_quantize_bf16", _p(x), _p(codes), _p(scales), rows, k, max(k, x.stride(0)), _stream())
+    return Mxfp4(codes, scales, rows, k)
+
+
+def mxfp4_dequantize(q: Mxfp4) -> torch.Tensor:
+    """The bf16 [rows, k] values that q stands for (exact)."""
+    _chk_mxfp4(q, "q")
+    with _same_device(q.codes.device, q.scales):
+        y = torch.empty((q.rows, q.k), dtype=_BF16, device=q.codes.device)
+        _lib.call("ea_mxfp4_dequantize_bf16", _p(q.codes), _p(q.scales), _p(y), q.rows, q.k, _stream())
+    return y
+
+
+def gemm_mxfp4(A: Union[torch.Tensor, Mxfp4], W: Mxfp4, bias: Optional[torch.Tensor], epilogue: int = EPI_BIAS,
+               out: Optional[torch.Tensor] = None, res: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[b] = epi(A[b] @ W.T + bias) over 4-bit operands, W of a [N, K] nn.Linear weight (N % 8 == 0).  A: bf16 [B, M, K] or [M, K]
+    (quantised here: mxfp4_quantize's values), or the Mxfp4 of [M, K].  bias fp32 [N]; out bf16 [B, M, N] (fp32 for EPI_F32_OUT); res
+    bf16 like out (may alias out); gate fp32 [B, N] ([N] for two-dimensional A); epilogues as gemm()."""
+    _chk_mxfp4(W, "W")
+    N, K = W.rows, W.k
+    packed = isinstance(A, Mxfp4)
+    if packed:
+        _chk_mxfp4(A, "A")
+        B, M, ak, squeeze, dev = 1, A.rows, A.k, True, A.codes.device
+    else:
+        _chk(A, _BF16, "A")
+        if A.dim() not in (2, 3):
+            raise ValueError(f"A: expected [M, K] or [B, M, K], got {tuple(A.shape)}")
+        squeeze, dev = A.dim() == 2, A.device
+        if squeeze:
+            A = A.unsqueeze(0)
+        B, M, ak = A.shape
+    if ak != K:
+        raise ValueError(f"A has K = {ak}, W has K = {K}")
+    if epilogue not in (EPI_BIAS, EPI_BIAS_GELU_TANH, EPI_BIAS_GATE_RES, EPI_F32_OUT):
+        raise ValueError(f"unknown epilogue {epilogue}")
+    if squeeze:
+        out = out.unsqueeze(0) if out is not None else None
+        res = res.unsqueeze(0) if res is not None else None
+        gate = gate.unsqueeze(0) if gate is not None and gate.dim() == 1 else gate
+    odt = _F32 if epilogue == EPI_F32_OUT else _BF16
+    with _same_device(dev, W.codes, W.scales, bias, out, res, gate, A.scales if packed else None):
+        if out is None:
+            out = torch.empty((B, M, N), dtype=odt, device=dev)
+        _chk(out, odt, "out")
+        if out.shape != (B, M, N) or out.stride(2) != 1:
+            raise ValueError(f"out: expected [{B}, {M}, {N}] with unit inner stride, got {tuple(out.shape)}, strides {out.stride()}")
+        if bias is not None:
+            _chk(bias, _F32, "bias")
+            if bias.shape != (N,) or not bias.is_contiguous():
+                raise ValueError(f"bias: expected contiguous [{N}], got {tuple(bias.shape)}")
+        ldres = rbs = gbs = 0
+        if epilogue == EPI_BIAS_GATE_RES:
+            if res is None or gate is None:
+                raise ValueError("EPI_BIAS_GATE_RES needs res and gate")
+            _chk(res, _BF16, "res"); _chk(gate, _F32, "gate")
+            if res.shape != (B, M, N) or res.stride(2) != 1 or gate.shape != (B, N) or gate.stride(1) != 1:
+                raise ValueError(f"res / gate: expected [{B}, {M}, {N}] / [{B}, {N}] with unit inner stride, got {tuple(res.shape)} / {tuple(gate.shape)}")
+            ldres, rbs, gbs = res.stride(1), res.stride(0), gate.stride(0)
+        if B * M:
+            x, lda, abs_ = None, 0, 0
+            if not packed:
+                # few rows: the product quantises them itself (one launch); else once, in front of it
+                if M <= 16 and K % 8 == 0 and A.stride(2) == 1 and A.stride(1) % 8 == 0 and A.stride(0) % 8 == 0 and A.data_ptr() % 16 == 0:
+                    x, lda, abs_ = A, A.stride(1), A.stride(0)
+                else:
+                    A = mxfp4_quantize(A.reshape(B * M, K))
+            need = _lib.load().ea_gemm_mxfp4_workspace_bytes(B, M, N, K)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            _timed("gemm", lambda: _lib.call("ea_gemm_mxfp4", None if x is not None else _p(A.codes), None if x is not None else _p(A.scales), _p(x),
+                                             _p(W.codes), _p(W.scales), _p(bias), _p(out), _p(res), _p(gate), B, M, N, K, lda, abs_,
+                                             out.stride(1), out.stride(0), ldres, rbs, gbs, int(epilogue), _p(ws), need, _stream()))
+    return out.squeeze(0) if squeeze else out
 
 
 # Softmax scale of head_dim 64 folded into Q (exp2 domain): q_scale = 64^-1/2 * log2(e) at ea_qknorm_rope_bf16, and
