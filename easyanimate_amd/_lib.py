@@ -58,6 +58,8 @@ PROTOTYPES = {
     "ea_rope_half_scatter_bf16": [_P, _P, _P, _P, _I, _I, _I, _I, _L, _P],
     "ea_silu_mul_bf16": [_P, _P, _P, _L, _I, _L, _L, _P],
     "ea_attention_causal_gqa_bf16": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P],
+    "ea_attention_text_workspace_bytes": [_I] * 7,
+    "ea_attention_text_bf16": [_P] * 5 + [_I] * 6 + [_F, _I, _F, _P, _I, _P, _P, _L, _L, _P, _P, _P, _P, _L, _P],
     "ea_tile_blend": [_P, _P, _I, _L, _I, _I, _L, _I, _L, _P],
     "ea_tile_corner_blend": [_P, _P, _I, _L, _I, _I, _I, _I, _P],
     "ea_conv3d_cl_bf16": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P],
@@ -97,6 +99,7 @@ def load() -> ctypes.CDLL:
     lib.ea_attention_state_bytes.restype = c_int64
     lib.ea_attention_state_bytes.argtypes = [c_int, c_int, c_int, c_int]
     lib.ea_gemm_mxfp4_workspace_bytes.restype = c_int64
+    lib.ea_attention_text_workspace_bytes.restype = c_int64
     lib.ea_conv3d_cl_tmerge_ok.restype = c_int
     lib.ea_conv3d_cl_tmerge_ok.argtypes = [c_int, c_int, c_int, c_int, c_int]
     lib.ea_conv3d_cl_blocked_ok.restype = c_int

@@ -1,0 +1,765 @@
+// Attention of text models: softmax(f(q k^T)) v with grouped-query heads, scores capped by a tanh and / or biased by distance, and any
+// combination of causal order, a prefix that every query sees, packed documents and key lengths:
+//     t = scale q.k;   t = cap tanh(t / cap);   t += bias[h][clamp(j - p, -R, R) + R]        p = q_start[b] + i, the query's position
+//     key j is visible to query i:  j < valid[b]  and  (not causal or j <= p or j < prefix[b])  and  kv_docs[b][j] == q_docs[b][i]
+// Order, prefix and length together are ONE limit per query -- keys j < lim(i) = min(valid, max(p + 1, prefix)) -- so a partly masked
+// tile costs one comparison per score, plus one when documents are packed.  A query that sees nothing yields zeros; what hidden keys
+// and values hold (NaN included) does not reach the result.
+//
+// A "row" is a (query, head of the group) pair: the heads that share a K / V head are packed next to each other (row = query * pack +
+// head), so a K / V tile serves all of them, a single new token fills a 16-row matrix tile as far as its group reaches, and a causal
+// tile's diagonal is `pack` times narrower in keys.
+//
+// Evaluated transposed as in the other attention kernels (S^T = K Q^T, O^T = V^T P^T on v_mfma_f32_16x16x32_bf16): a lane owns one row
+// and, because K rows are fed in the order 8 (r / 4) + 4 kt + r % 4, eight consecutive keys of a 32-key block = its slice of the P^T
+// operand.  V stays row-major in memory and LDS; its transposed fragments come from ds_read_b64_tr_b16.  One pass with a running
+// maximum that is only moved when a score exceeds it by 2^8 (P then stays below 256 -- bf16 has fp32's exponent range -- and the
+// accumulators are hardly ever rescaled); P is rounded to bf16 for its product (2^-9 of each weight), the row sums are fp32 of the
+// unrounded weights.
+//
+//   attention_text_kernel       128 rows per workgroup (four waves, 32 rows each), K / V tiles of 64 keys double-buffered in LDS by
+//                               LDS-DMA; tiles that no row of the workgroup sees are skipped (64 at a time for documents)
+//   attention_text_few_kernel   up to 16 rows: each of the four waves walks its own 32-key blocks, K straight into registers
+//   Both can split the keys over workgroups; attention_text_join_kernel combines the partial results in a fixed order.
+#include "ea_common.h"
+
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2_a __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4_a __attribute__((ext_vector_type(4)));
+
+struct TextArgs {
+    const unsigned short* q;
+    const unsigned short* k;
+    const unsigned short* v;
+    unsigned short* out;
+    const float* bias;        // [Hq][2 reach + 1] or null
+    const int* q_docs;        // [B][Sq] (row stride qd_ld) or null
+    const int* kv_docs;       // [B][Sk]
+    const int* doc_range;     // [B][key tiles][2]: least and greatest document of each 64-key tile
+    const int* prefix;        // [B] or null
+    const int* valid;         // [B] or null
+    const int* q_start;       // [B] or null (Sk - Sq)
+    float* part;              // [splits][rows][D] and, behind it, [splits][rows][2] = (running maximum, sum)
+    int64_t qb, qh, qs, kb, kh, ks, vb, vh, vs, ob, os, qd_ld, kd_ld;
+    int B, Hq, Hkv, Sq, Sk, group, pack, causal, reach, splits, row_tiles, key_tiles;
+    float scale, cap;
+};
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr int BIAS_PACK_MAX = 16;       // heads packed into a row tile at most (bounds the bias window: see bias_window)
+
+__device__ __forceinline__ void glds16t(const void* gptr, void* lds_wave_base) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gptr,
+                                     (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
+}
+
+// 16-byte-chunk swizzles of the LDS rows (2 D bytes each).  K fragments read rows {0..3, 8..11, ..} of a block eight lanes at a time:
+// all different in the low three bits.  V's transposed reads take 32-byte pieces of rows {0..3} of every 8: the piece index moves.
+template <int D>
+__device__ __forceinline__ int k_swz(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
+template <int D>
+__device__ __forceinline__ int v_swz(int row) {
+    return D == 128 ? 2 * ((row & 3) | ((row >> 3) & 1) << 2) : 2 * (((row >> 1) & 1) | ((row >> 3) & 1) << 1);
+}
+
+// ---- the rows of one wave -------------------------------------------------------------------------------------------------------
+template <int D, int RT>
+struct Rows {
+    bf16x8 q[RT][D / 32];
+    int64_t out_off[RT];      // element offset of the row's output, -1: no such row
+    int lim[RT], doc[RT];     // keys below lim (and of the row's document) are visible
+    int back[RT];             // distance bias: (last query of the tile) - (this query), + the row's head's window
+    int lim_lo, lim_hi;       // over the wave's rows
+    int doc_lo, doc_hi;
+    f32x4 o[RT][D / 16];
+    float m[RT], l[RT];       // the reference maximum (log2 domain), this lane's share of the sum
+};
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ int64_t first_position(const TextArgs& p, int b) { return p.q_start ? p.q_start[b] : (int64_t)p.Sk - p.Sq; }
+__device__ __forceinline__ int key_limit(const TextArgs& p, int b, int qi) {
+    int64_t lim = p.Sk;
+    if (p.valid) lim = p.valid[b] < lim ? p.valid[b] : lim;
+    if (p.causal) {
+        int64_t c = first_position(p, b) + qi + 1;
+        if (p.prefix && p.prefix[b] > c) c = p.prefix[b];
+        lim = c < lim ? c : lim;
+    }
+    return lim > 0 ? (int)lim : 0;
+}
+
+// head0: first query head of the packed set; row0: first row of this wave; qlast: last query of the workgroup's tile
+template <int D, int RT>
+__device__ __forceinline__ void load_rows(const TextArgs& p, Rows<D, RT>& R, int b, int head0, int row0, int qlast, int win, int lane) {
+    const int lr = lane & 15, lq = lane >> 4;
+    R.lim_lo = 0x7fffffff;
+    R.lim_hi = 0;
+    R.doc_lo = 0x7fffffff;
+    R.doc_hi = -0x7fffffff - 1;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int row = row0 + t * 16 + lr;
+        int qi = row / p.pack;
+        const bool live = qi < p.Sq;
+        const int hg = live ? row % p.pack : p.pack - 1;
+        qi = live ? qi : p.Sq - 1;                        // rows past the end repeat the last one and are not stored
+        const unsigned short* src = p.q + b * p.qb + (int64_t)(head0 + hg) * p.qh + (int64_t)qi * p.qs + lq * 8;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) R.q[t][s] = *reinterpret_cast<const bf16x8*>(src + s * 32);
+        R.out_off[t] = live ? b * p.ob + (int64_t)qi * p.os + (int64_t)(head0 + hg) * D : -1;
+        R.lim[t] = key_limit(p, b, qi);
+        R.doc[t] = p.q_docs ? p.q_docs[b * p.qd_ld + qi] : 0;
+        R.back[t] = hg * win + (qlast - qi);
+        R.lim_lo = min(R.lim_lo, R.lim[t]);
+        R.lim_hi = max(R.lim_hi, R.lim[t]);
+        R.doc_lo = min(R.doc_lo, R.doc[t]);
+        R.doc_hi = max(R.doc_hi, R.doc[t]);
+        R.m[t] = NEG_INF;
+        R.l[t] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) R.o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    R.lim_lo = __builtin_amdgcn_readfirstlane(wave_min(R.lim_lo));
+    R.lim_hi = __builtin_amdgcn_readfirstlane(wave_max(R.lim_hi));
+    if (p.q_docs) {
+        R.doc_lo = __builtin_amdgcn_readfirstlane(wave_min(R.doc_lo));
+        R.doc_hi = __builtin_amdgcn_readfirstlane(wave_max(R.doc_hi));
+    }
+}
+
+// cap tanh(t / cap) log2(e) of t = s scale.  tanh(x) = 1 - 2 / (1 + e^2x): absolute error about cap 2^-22, so for a cap that is large
+// beside the scores (cap_wide: cap > 256) small x go through the odd series x - x^3/3 + 2x^5/15 - 17x^7/315 (|x| < 0.25: the next
+// term is 6e-8 of x) instead.
+__device__ __forceinline__ float capped_log2(float s, float two_over, float c1, float half_over, bool wide) {
+    const float e = __builtin_amdgcn_exp2f(s * two_over);
+    float t = __builtin_fmaf(-2.0f * c1, __builtin_amdgcn_rcpf(e + 1.0f), c1);
+    if (wide) {
+        const float x = s * half_over, x2 = x * x;
+        const float series = x * __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+        t = fabsf(x) < 0.25f ? c1 * series : t;
+    }
+    return t;
+}
+
+// One 32-key block: scores of the wave's rows, softmax update, product with V.
+//   kf: its K fragments; vt: LDS byte address of this lane's transposed V reads (vtile + v_row_base); key0: its first key
+//   masked: some pair of the block may be hidden;  docs: this lane's 8 keys' documents (masked blocks of packed rows)
+//   win0: this lane's bias window position of key 8 lq of the block (bias variant)
+template <int D, int RT, bool CAP, bool BIAS>
+__device__ __forceinline__ void block_step(const TextArgs& p, Rows<D, RT>& R, const bf16x8 (&kf)[2][D / 32], const char* vtile, int key0, bool masked,
+                                           const int (&docs)[8], const float* win0, int lane) {
+    constexpr int NT = D / 16;
+    const int lr = lane & 15, lq = lane >> 4;
+    const float c = p.scale * LOG2E;
+    float s[RT][8];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks) a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kt][ks], R.q[t][ks], a, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][kt * 4 + r] = a[r];
+        }
+    // ---- to the log2 domain where a cap or a bias makes the score more than a multiple of q.k; hidden pairs to -inf
+    float unit = c;                    // what a score still has to be multiplied with
+    if (CAP) {
+        const float c1 = p.cap * LOG2E, two_over = 2.0f * c / p.cap, half_over = p.scale / p.cap;
+        const bool wide = p.cap > 256.0f;
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[t][e] = capped_log2(s[t][e], two_over, c1, half_over, wide);
+        unit = 1.0f;
+    }
+    if (BIAS) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[t][e] = __builtin_fmaf(s[t][e], unit, win0[R.back[t] + e]);
+        unit = 1.0f;
+    }
+    if (masked) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                bool see = key0 + 8 * lq + e < R.lim[t];
+                if (p.q_docs) see = see && docs[e] == R.doc[t];
+                s[t][e] = see ? s[t][e] : NEG_INF;
+            }
+    }
+    // ---- move the reference maximum only when a row has outgrown it
+    float top[RT];
+    bool grow = false;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        top[t] = fmaxf(fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])), fmaxf(fmaxf(s[t][4], s[t][5]), fmaxf(s[t][6], s[t][7]))) * unit;
+        grow = grow || top[t] > R.m[t] + 8.0f;
+    }
+    if (__ballot(grow)) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            float n = fmaxf(top[t], __shfl_xor(top[t], 16, 64));
+            n = fmaxf(n, __shfl_xor(n, 32, 64));
+            n = fmaxf(n, R.m[t]);
+            const float alpha = n == NEG_INF ? 1.0f : __builtin_amdgcn_exp2f(R.m[t] - n);
+            R.m[t] = n;
+            R.l[t] *= alpha;
+#pragma unroll
+            for (int d = 0; d < NT; ++d) R.o[t][d] *= alpha;
+        }
+    }
+    bf16x8 pb[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const float ref = R.m[t] == NEG_INF ? 0.0f : R.m[t];
+        u32x4_a pk;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], unit, -ref));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e + 1], unit, -ref));
+            R.l[t] += p0 + p1;
+            const f32x2 two = {p0, p1};
+            pk[e >> 1] = __builtin_bit_cast(unsigned, __builtin_convertvector(two, bf16x2));
+        }
+        pb[t] = __builtin_bit_cast(bf16x8, pk);
+    }
+    // ---- O^T += V^T P^T.  Lane (lr, lq) of a transposed read: keys 8 lq + (0..3 | 4..7), columns 16 d + lr.
+    const int vrow = 8 * lq + (lr >> 2);
+#pragma unroll
+    for (int d = 0; d < NT; ++d) {
+        const int ch = ((2 * d + ((lr & 3) >> 1)) ^ v_swz<D>(vrow)) * 16 + (lr & 1) * 8;     // (+ 4 rows: the same swizzle)
+        const char* a = vtile + vrow * (2 * D) + ch;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 4 * (2 * D)));
+        u32x4_a vw;
+        const u32x2_a l2 = __builtin_bit_cast(u32x2_a, lo), h2 = __builtin_bit_cast(u32x2_a, hi);
+        vw[0] = l2[0]; vw[1] = l2[1]; vw[2] = h2[0]; vw[3] = h2[1];
+        if (masked) {
+            // a hidden key's weight is 0, but 0 times NaN or infinity is not: such elements of V are taken out of the matrix product
+            // (and added below for the rows that do see them)
+            unsigned odd = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const bool b0 = (vw[w] & 0x7f80u) == 0x7f80u, b1 = (vw[w] & 0x7f800000u) == 0x7f800000u;
+                odd |= (b0 || b1) ? 1u : 0u;
+                vw[w] = (b0 ? 0u : vw[w] & 0xffffu) | (b1 ? 0u : vw[w] & 0xffff0000u);
+            }
+            if (__ballot(odd)) {
+                for (int key = 0; key < 32; ++key) {
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) {
+                        const u32x4_a pw = __builtin_bit_cast(u32x4_a, pb[t]);
+                        const int src = (key >> 3) * 16 + lr;                                // the lane that holds this row's weight
+                        const unsigned word = (key & 6) == 0 ? pw[0] : (key & 6) == 2 ? pw[1] : (key & 6) == 4 ? pw[2] : pw[3];
+                        const unsigned w = __shfl((int)word, src, 64);
+                        const bool seen = ((key & 1 ? w >> 16 : w) & 0x7fffu) != 0;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int col = 16 * d + lq * 4 + r;
+                            const unsigned short bits = *reinterpret_cast<const unsigned short*>(
+                                vtile + key * (2 * D) + (((col >> 3) ^ v_swz<D>(key)) << 4) + (col & 7) * 2);
+                            if (seen && (bits & 0x7f80) == 0x7f80) R.o[t][d][r] += bf16_bits_to_f32(bits);
+                        }
+                    }
+                }
+            }
+        }
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, vw);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) R.o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[t], R.o[t][d], 0, 0, 0);
+    }
+}
+
+// ---- which key tiles a workgroup visits ------------------------------------------------------------------------------------------
+// Tiles [lo, hi); with documents only those whose range of documents meets [dlo, dhi]: 64 tiles are looked up at once, one per lane.
+struct TileWalk {
+    const int* range;      // this batch element's [tiles][2], or null
+    int base, hi, dlo, dhi;
+    unsigned long long left;
+    int blo, bhi;          // the documents of the lane's tile in the current batch of 64
+    __device__ __forceinline__ void fill(int from, int lane) {
+        const int t = base + lane;
+        bool want = t >= from && t < hi;
+        blo = dlo; bhi = dlo;
+        if (range && want) {
+            blo = range[2 * t];
+            bhi = range[2 * t + 1];
+            want = blo <= dhi && bhi >= dlo;
+        }
+        left = __ballot(want);
+    }
+    __device__ __forceinline__ void start(int lo, int hi_, int lane) {
+        hi = hi_;
+        base = lo;
+        left = 0;
+        if (lo < hi) fill(lo, lane);
+    }
+    // the next tile, or -1; its documents' range goes to (lo, hi_)
+    __device__ __forceinline__ int next(int lane, int& lo, int& hi_) {
+        while (left == 0) {
+            base += 64;
+            if (base >= hi) return -1;
+            fill(base, lane);
+        }
+        const int i = __builtin_ctzll(left);
+        left &= left - 1;
+        lo = __builtin_amdgcn_readlane(blo, i);
+        hi_ = __builtin_amdgcn_readlane(bhi, i);
+        return base + i;
+    }
+};
+
+// normalise and store the wave's rows, or leave its state for the join
+template <int D, int RT>
+__device__ __forceinline__ void store_rows(const TextArgs& p, Rows<D, RT>& R, int64_t part_row0, int split, int64_t rows_all, int row0, int lane) {
+    const int lr = lane & 15, lq = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        float l = R.l[t] + __shfl_xor(R.l[t], 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (R.out_off[t] < 0) continue;
+        if (p.splits == 1) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+                bf16x4 v;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = (bf16_t)(l == 0.0f ? 0.0f : R.o[t][d][r] * inv);
+                *reinterpret_cast<bf16x4*>(p.out + R.out_off[t] + d * 16 + lq * 4) = v;
+            }
+        } else {
+            const int64_t row = (int64_t)split * rows_all + part_row0 + row0 + t * 16 + lr;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(p.part + row * D + d * 16 + lq * 4) = R.o[t][d];
+            if (lq == 0) {
+                float* ml = p.part + (int64_t)p.splits * rows_all * D + row * 2;
+                ml[0] = R.m[t];
+                ml[1] = l;
+            }
+        }
+    }
+}
+
+// ---- 128 rows per workgroup ------------------------------------------------------------------------------------------------------
+constexpr int TROWS = 128, TKEYS = 64;
+// floats per head of a tile's bias window: its 64 keys against every query of the row tile
+__host__ __device__ __forceinline__ int bias_window(int pack) { return TKEYS + (TROWS - 1) / pack + 2; }
+
+template <int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int OPER = TKEYS * 2 * D;                 // one operand tile, bytes
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lr = lane & 15, lq = lane >> 4;
+    // heads vary fastest, long (late) row tiles first: workgroups of one K / V head tend to share an XCD, causal work is dealt evenly
+    const int nsets = p.Hq / p.pack;                    // packed head sets per batch element
+    const int set_all = blockIdx.x % (nsets * p.B), tile = p.row_tiles - 1 - blockIdx.x / (nsets * p.B);
+    const int b = set_all / nsets, set = set_all % nsets;
+    const int head0 = set * p.pack, hk = head0 / p.group;
+    const int split = blockIdx.y;
+    const int rows = p.Sq * p.pack;
+    const int q_first = tile * TROWS / p.pack;
+    const int q_last = min((tile * TROWS + TROWS - 1) / p.pack, p.Sq - 1);
+    const int win = BIAS ? bias_window(p.pack) : 1;
+
+    Rows<D, 2> R;
+    load_rows<D, 2>(p, R, b, head0, tile * TROWS + wave * 32, q_last, win, lane);
+
+    // ---- the workgroup's keys: up to the greatest limit (the limit grows with the query), documents of its queries
+    const int lim_all = key_limit(p, b, q_last);
+    const int nt = (lim_all + TKEYS - 1) / TKEYS;
+    TileWalk walk;
+    walk.range = nullptr;
+    walk.dlo = walk.dhi = 0;
+    if (p.q_docs) {
+        int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+        for (int i = q_first + lane; i <= q_last; i += 64) {
+            const int id = p.q_docs[b * p.qd_ld + i];
+            lo = min(lo, id);
+            hi = max(hi, id);
+        }
+        walk.dlo = __builtin_amdgcn_readfirstlane(wave_min(lo));
+        walk.dhi = __builtin_amdgcn_readfirstlane(wave_max(hi));
+        walk.range = p.doc_range + (int64_t)b * p.key_tiles * 2;
+    }
+    walk.start((int)((int64_t)nt * split / p.splits), (int)((int64_t)nt * (split + 1) / p.splits), lane);
+
+    const unsigned short* Kh = p.k + b * p.kb + (int64_t)hk * p.kh;
+    const unsigned short* Vh = p.v + b * p.vb + (int64_t)hk * p.vh;
+    constexpr int PER = 64 / (D / 8), PIECES = TKEYS / PER / 4;       // rows per 1 KiB piece, pieces per wave and operand
+    auto issue = [&](int t, int stage) {
+        char* ks = smem + stage * 2 * OPER + wave * PIECES * 1024;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = (wave * PIECES + i) * PER + lane / (D / 8), cs = lane % (D / 8);
+            int key = t * TKEYS + r;
+            key = key < p.Sk ? key : p.Sk - 1;
+            glds16t(Kh + (int64_t)key * p.ks + ((cs ^ k_swz<D>(r)) << 3), ks + i * 1024);
+            glds16t(Vh + (int64_t)key * p.vs + ((cs ^ v_swz<D>(r)) << 3), ks + OPER + i * 1024);
+        }
+    };
+    // bias window of tile t: entry w of head g = bias at distance 64 t - position(q_last) + w, in the log2 domain.  Finite values stay
+    // finite there (the lowest float times log2 e would not): rows that are biased down as a whole keep their order.
+    float* wins = reinterpret_cast<float*>(smem + 4 * OPER);
+    const int64_t p_last = first_position(p, b) + q_last;
+    auto stage_bias = [&](int t, int stage) {
+        float* dst = wins + stage * p.pack * win;
+        for (int i = tid; i < p.pack * win; i += 256) {
+            const int g = i / win, w = i - g * win;
+            int64_t dist = (int64_t)t * TKEYS - p_last + w;
+            dist = dist < -p.reach ? -p.reach : dist > p.reach ? p.reach : dist;
+            const float v = p.bias[(int64_t)(head0 + g) * (2 * p.reach + 1) + p.reach + (int)dist];
+            const float big = 3.4028234663852886e38f;
+            dst[i] = fabsf(v) <= big ? fminf(fmaxf(v * LOG2E, -big), big) : v;
+        }
+    };
+
+    int dlo, dhi, nlo = 0, nhi = 0;
+    int t = walk.next(lane, dlo, dhi);
+    int stage = 0;
+    if (t >= 0) {
+        issue(t, 0);
+        if (BIAS) stage_bias(t, 0);
+    }
+    while (t >= 0) {
+        const int tn = walk.next(lane, nlo, nhi);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (tn >= 0) {
+            issue(tn, stage ^ 1);
+            if (BIAS) stage_bias(tn, stage ^ 1);
+        }
+        const char* kt0 = smem + stage * 2 * OPER;
+        const int key0 = t * TKEYS;
+        const bool mine = key0 < R.lim_hi && (!p.q_docs || (dlo <= R.doc_hi && dhi >= R.doc_lo));
+        if (mine) {
+            const bool masked = !(key0 + TKEYS <= R.lim_lo && (!p.q_docs || (dlo == dhi && R.doc_lo == R.doc_hi && dlo == R.doc_lo)));
+#pragma unroll
+            for (int blk = 0; blk < 2; ++blk) {
+                bf16x8 kf[2][D / 32];
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt) {
+                    const int row = blk * 32 + 8 * (lr >> 2) + 4 * kt + (lr & 3);
+#pragma unroll
+                    for (int s = 0; s < D / 32; ++s)
+                        kf[kt][s] = *reinterpret_cast<const bf16x8*>(kt0 + row * (2 * D) + (((s * 4 + lq) ^ k_swz<D>(row)) << 4));
+                }
+                int docs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (masked && p.q_docs) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int key = key0 + blk * 32 + 8 * lq + e;
+                        docs[e] = p.kv_docs[b * p.kd_ld + (key < p.Sk ? key : p.Sk - 1)];
+                    }
+                }
+                block_step<D, 2, CAP, BIAS>(p, R, kf, kt0 + OPER + blk * 32 * (2 * D), key0 + blk * 32, masked, docs,
+                                            wins + stage * p.pack * win + blk * 32 + 8 * lq, lane);
+            }
+        }
+        t = tn;
+        dlo = nlo;
+        dhi = nhi;
+        stage ^= 1;
+    }
+    store_rows<D, 2>(p, R, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, tile * TROWS + wave * 32, lane);
+}
+
+// ---- up to 16 rows: the keys are what is long -----------------------------------------------------------------------------------
+// Wave w of split s takes the 32-key blocks w, w + 4, .. of the split's range; its K fragments come straight from memory into registers
+// (a row's 2 D bytes are read whole), its V block through a private double buffer in LDS.  No barrier until the four states are joined.
+template <int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int OPER = 32 * 2 * D;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 15, lq = lane >> 4;
+    const int nsets = p.Hq / p.pack;
+    const int set_all = blockIdx.x % (nsets * p.B);
+    const int b = set_all / nsets, set = set_all % nsets;
+    const int head0 = set * p.pack, hk = head0 / p.group;
+    const int split = blockIdx.y;
+    const int rows = p.Sq * p.pack;
+    const int win = BIAS ? bias_window(p.pack) : 1;
+
+    Rows<D, 1> R;
+    load_rows<D, 1>(p, R, b, head0, 0, p.Sq - 1, win, lane);
+    const int nb = (key_limit(p, b, p.Sq - 1) + 31) / 32;
+    const int b0 = (int)((int64_t)nb * split / p.splits), b1 = (int)((int64_t)nb * (split + 1) / p.splits);
+
+    const unsigned short* Kh = p.k + b * p.kb + (int64_t)hk * p.kh;
+    const unsigned short* Vh = p.v + b * p.vb + (int64_t)hk * p.vh;
+    char* const mine = smem + wave * 2 * OPER;
+    float* const win_mine = reinterpret_cast<float*>(smem + 8 * OPER) + wave * p.pack * win;
+    const int64_t p_last = first_position(p, b) + p.Sq - 1;
+    constexpr int PER = 64 / (D / 8), PIECES = 32 / PER;
+    auto load_k = [&](int blk, bf16x8 (&kf)[2][D / 32]) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            int key = blk * 32 + 8 * (lr >> 2) + 4 * kt + (lr & 3);
+            key = key < p.Sk ? key : p.Sk - 1;
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) kf[kt][s] = *reinterpret_cast<const bf16x8*>(Kh + (int64_t)key * p.ks + (s * 4 + lq) * 8);
+        }
+    };
+    auto load_v = [&](int blk, int stage) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int r = i * PER + lane / (D / 8), cs = lane % (D / 8);
+            int key = blk * 32 + r;
+            key = key < p.Sk ? key : p.Sk - 1;
+            glds16t(Vh + (int64_t)key * p.vs + ((cs ^ v_swz<D>(r)) << 3), mine + stage * OPER + i * 1024);
+        }
+    };
+    bf16x8 kf[2][D / 32];
+    int blk = b0 + wave, stage = 0;
+    if (blk < b1) {
+        load_k(blk, kf);
+        load_v(blk, 0);
+    }
+    for (; blk < b1; blk += 4, stage ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        bf16x8 now[2][D / 32];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) now[kt][s] = kf[kt][s];
+        if (blk + 4 < b1) {
+            load_k(blk + 4, kf);
+            load_v(blk + 4, stage ^ 1);
+        }
+        const int key0 = blk * 32;
+        if (BIAS) {
+            const int span = p.Sq - 1;           // this block's window: 32 keys against every query
+            for (int i = lane; i < p.pack * win; i += 64) {
+                const int g = i / win, w = i - g * win;
+                if (w < 32 + span) {
+                    int64_t dist = (int64_t)key0 - p_last + w;
+                    dist = dist < -p.reach ? -p.reach : dist > p.reach ? p.reach : dist;
+                    const float v = p.bias[(int64_t)(head0 + g) * (2 * p.reach + 1) + p.reach + (int)dist];
+                    const float big = 3.4028234663852886e38f;
+                    win_mine[i] = fabsf(v) <= big ? fminf(fmaxf(v * LOG2E, -big), big) : v;
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        int docs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const bool masked = key0 + 32 > R.lim_lo || p.q_docs;
+        if (p.q_docs) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int key = key0 + 8 * lq + e;
+                docs[e] = p.kv_docs[b * p.kd_ld + (key < p.Sk ? key : p.Sk - 1)];
+            }
+        }
+        block_step<D, 1, CAP, BIAS>(p, R, now, mine + stage * OPER, key0, masked, docs, win_mine + 8 * lq, lane);
+    }
+    // ---- join the four waves' states through LDS: wave 0 takes the others in their order
+    __syncthreads();
+    constexpr int NT = D / 16;
+    f32x4* const ox = reinterpret_cast<f32x4*>(smem);                  // [3][NT][64]: 3 x 16 x D floats, inside the V buffers
+    float* const mx = reinterpret_cast<float*>(smem + 3 * NT * 64 * 16);   // [3][2][64]
+    if (wave > 0) {
+#pragma unroll
+        for (int d = 0; d < NT; ++d) ox[((wave - 1) * NT + d) * 64 + lane] = R.o[0][d];
+        mx[(wave - 1) * 128 + lane] = R.m[0];
+        mx[(wave - 1) * 128 + 64 + lane] = R.l[0];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) {
+        const float m2 = mx[w * 128 + lane], l2 = mx[w * 128 + 64 + lane];
+        const float n = fmaxf(R.m[0], m2), ref = n == NEG_INF ? 0.0f : n;
+        const float a1 = __builtin_amdgcn_exp2f(R.m[0] - ref), a2 = __builtin_amdgcn_exp2f(m2 - ref);
+        R.m[0] = n;
+        R.l[0] = R.l[0] * a1 + l2 * a2;
+#pragma unroll
+        for (int d = 0; d < NT; ++d) R.o[0][d] = R.o[0][d] * a1 + ox[(w * NT + d) * 64 + lane] * a2;
+    }
+    store_rows<D, 1>(p, R, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, 0, lane);
+}
+
+// one wave per row: the splits' states in their order
+template <int D>
+__global__ __launch_bounds__(256) void attention_text_join_kernel(TextArgs p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t rows_all = (int64_t)p.B * p.Hq * p.Sq;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows_all) return;
+    const float* ml = p.part + (int64_t)p.splits * rows_all * D;
+    float top = NEG_INF;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[(s * rows_all + row) * 2]);
+    const float ref = top == NEG_INF ? 0.0f : top;
+    float l = 0.f, o[D / 64];
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+        const int64_t r = s * rows_all + row;
+        const float a = __builtin_amdgcn_exp2f(ml[r * 2] - ref);
+        l += ml[r * 2 + 1] * a;
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) o[e] += p.part[r * D + e * 64 + lane] * a;
+    }
+    // row = ((b * sets + set) * Sq + query) * pack + head of the set
+    const int64_t rows = (int64_t)p.Sq * p.pack;
+    const int nsets = p.Hq / p.pack;
+    const int64_t set_all = row / rows;
+    const int in = (int)(row - set_all * rows), qi = in / p.pack, hg = in % p.pack;
+    const int64_t b = set_all / nsets;
+    const int head = (int)(set_all % nsets) * p.pack + hg;
+    unsigned short* dst = p.out + b * p.ob + (int64_t)qi * p.os + (int64_t)head * D;
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) dst[e * 64 + lane] = f32_to_bf16_bits(l == 0.0f ? 0.0f : o[e] / l);
+}
+
+// least and greatest document of every 64-key tile: one wave each
+__global__ __launch_bounds__(64) void doc_range_kernel(const int* __restrict__ docs, int* __restrict__ range, int64_t ld, int Sk, int tiles) {
+    const int t = blockIdx.x, b = blockIdx.y;
+    int key = t * 64 + (int)threadIdx.x;
+    key = key < Sk ? key : Sk - 1;
+    const int id = docs[b * ld + key];
+    const int lo = wave_min(id), hi = wave_max(id);
+    if (threadIdx.x == 0) {
+        range[((int64_t)b * tiles + t) * 2] = lo;
+        range[((int64_t)b * tiles + t) * 2 + 1] = hi;
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------------
+struct Plan {
+    int group, pack, few, row_tiles, key_tiles, splits;
+    int64_t part_bytes, range_bytes;
+};
+
+Plan plan_of(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs) {
+    Plan n;
+    n.group = Hq / Hkv;
+    n.pack = n.group < BIAS_PACK_MAX ? n.group : BIAS_PACK_MAX;
+    while (n.group % n.pack) --n.pack;                    // the largest divisor of the group up to BIAS_PACK_MAX
+    const int64_t rows = (int64_t)Sq * n.pack;
+    const int64_t sets = (int64_t)B * (Hq / n.pack);
+    n.few = rows <= 16;
+    n.key_tiles = (int)(((int64_t)Sk + TKEYS - 1) / TKEYS);
+    n.row_tiles = n.few ? 1 : (int)((rows + TROWS - 1) / TROWS);
+    // split the keys while the workgroups do not fill the chip twice (256 CUs) and a split keeps at least 256 keys
+    const int64_t wgs = sets * n.row_tiles;
+    int64_t s = (512 + wgs - 1) / wgs;
+    const int64_t most = ((int64_t)Sk + 255) / 256;
+    s = s < most ? s : most;
+    s = s < 1 ? 1 : s > 256 ? 256 : s;
+    if (!n.few && wgs >= 192) s = 1;
+    n.splits = (int)s;
+    n.part_bytes = n.splits > 1 ? n.splits * sets * rows * (D + 2) * 4 : 0;
+    n.range_bytes = docs && !n.few ? (int64_t)B * n.key_tiles * 8 : 0;
+    return n;
+}
+
+template <int D, bool CAP, bool BIAS>
+int launch_text(const TextArgs& p, const Plan& n, hipStream_t st) {
+    const int oper = (n.few ? 32 : TKEYS) * 2 * D;
+    const int win = BIAS ? bias_window(p.pack) * p.pack * 4 : 0;
+    const int64_t sets = (int64_t)p.B * (p.Hq / p.pack);
+    if (n.few) {
+        const int tail = 3 * 16 * D * 4 + 3 * 2 * 64 * 4;                 // the join's image
+        int lds = 8 * oper + 4 * win;
+        lds = lds > tail ? lds : tail;
+        if (hipFuncSetAttribute((const void*)attention_text_few_kernel<D, CAP, BIAS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+            return ea_check_launch("ea_attention_text_bf16");
+        ea_count("attention_text_few");
+        hipLaunchKernelGGL((attention_text_few_kernel<D, CAP, BIAS>), dim3((unsigned)sets, (unsigned)n.splits), dim3(256), lds, st, p);
+    } else {
+        const int lds = 4 * oper + 2 * win;
+        if (hipFuncSetAttribute((const void*)attention_text_kernel<D, CAP, BIAS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+            return ea_check_launch("ea_attention_text_bf16");
+        ea_count(n.splits > 1 ? "attention_text_split" : "attention_text");
+        hipLaunchKernelGGL((attention_text_kernel<D, CAP, BIAS>), dim3((unsigned)(sets * n.row_tiles), (unsigned)n.splits), dim3(256), lds, st, p);
+    }
+    if (n.splits > 1) {
+        const int64_t rows_all = (int64_t)p.B * p.Hq * p.Sq;
+        hipLaunchKernelGGL(attention_text_join_kernel<D>, dim3((unsigned)((rows_all + 3) / 4)), dim3(256), 0, st, p);
+    }
+    return ea_check_launch("ea_attention_text_bf16");
+}
+
+template <int D>
+int dispatch_text(const TextArgs& p, const Plan& n, hipStream_t st) {
+    if (p.cap > 0.0f) return p.bias ? launch_text<D, true, true>(p, n, st) : launch_text<D, true, false>(p, n, st);
+    return p.bias ? launch_text<D, false, true>(p, n, st) : launch_text<D, false, false>(p, n, st);
+}
+
+bool sizes_ok(int B, int Hq, int Hkv, int Sq, int Sk, int D) {
+    if (!(B > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Sq >= 0 && Sk >= 0 && (D == 64 || D == 128))) return false;
+    // rows of a packed set stay in 32 bits, grids within a launch's limits
+    return (int64_t)Sq * BIAS_PACK_MAX <= 0x7fffff00 && Sk <= 0x7fffff00 && B <= 65535 && (int64_t)B * Hq * (((int64_t)Sq + 7) / 8) <= 0x7fffffff;
+}
+
+}  // namespace
+
+extern "C" int64_t ea_attention_text_workspace_bytes(int batch, int q_heads, int kv_heads, int q_len, int kv_len, int head_dim, int documents) {
+    if (!sizes_ok(batch, q_heads, kv_heads, q_len, kv_len, head_dim) || q_len == 0 || kv_len == 0) return 0;
+    const Plan n = plan_of(batch, q_heads, kv_heads, q_len, kv_len, head_dim, documents);
+    return n.part_bytes + n.range_bytes;
+}
+
+extern "C" int ea_attention_text_bf16(const ea_bf16* q, const ea_bf16* k, const ea_bf16* v, ea_bf16* out, const int64_t* strides, int batch,
+                                      int q_heads, int kv_heads, int q_len, int kv_len, int head_dim, float scale, int causal, float cap,
+                                      const float* bias, int reach, const int* q_docs, const int* kv_docs, int64_t q_docs_ld, int64_t kv_docs_ld,
+                                      const int* prefix, const int* valid, const int* q_start, void* workspace, int64_t workspace_bytes,
+                                      void* stream) {
+    EA_REQUIRE(head_dim == 64 || head_dim == 128, "ea_attention_text_bf16: head_dim %d (64 and 128 are built)", head_dim);
+    EA_REQUIRE(sizes_ok(batch, q_heads, kv_heads, q_len, kv_len, head_dim),
+               "ea_attention_text_bf16: bad sizes (batch %d, heads %d / %d, queries %d, keys %d)", batch, q_heads, kv_heads, q_len, kv_len);
+    EA_REQUIRE(scale > 0.0f && scale <= 3.4e38f, "ea_attention_text_bf16: scale must be positive and finite");
+    EA_REQUIRE(cap >= 0.0f && cap <= 3.4e38f, "ea_attention_text_bf16: cap must be positive and finite, or 0 for none");
+    EA_REQUIRE(!bias || (reach >= 0 && reach <= 0x3fffffff), "ea_attention_text_bf16: bad reach %d", reach);
+    EA_REQUIRE((q_docs == nullptr) == (kv_docs == nullptr), "ea_attention_text_bf16: q_docs and kv_docs come together");
+    EA_REQUIRE(!prefix || causal, "ea_attention_text_bf16: a prefix needs causal order");
+    if (q_len == 0) return EA_OK;
+    EA_REQUIRE(kv_len > 0, "ea_attention_text_bf16: no keys");
+    EA_REQUIRE(q && k && v && out && strides, "ea_attention_text_bf16: null tensor");
+    EA_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0, "ea_attention_text_bf16: 16-byte alignment");
+    for (int i = 0; i < 11; ++i)
+        EA_REQUIRE(strides[i] % 8 == 0 && strides[i] >= 0, "ea_attention_text_bf16: strides must be non-negative multiples of 8 elements");
+    const Plan n = plan_of(batch, q_heads, kv_heads, q_len, kv_len, head_dim, q_docs != nullptr);
+    EA_REQUIRE(n.part_bytes + n.range_bytes == 0 ||
+                   (workspace && workspace_bytes >= n.part_bytes + n.range_bytes && (uintptr_t)workspace % 16 == 0),
+               "ea_attention_text_bf16: needs %lld bytes of 16-byte aligned workspace (ea_attention_text_workspace_bytes)",
+               (long long)(n.part_bytes + n.range_bytes));
+    TextArgs p;
+    p.q = q; p.k = k; p.v = v; p.out = out; p.bias = bias; p.q_docs = q_docs; p.kv_docs = kv_docs; p.prefix = prefix; p.valid = valid;
+    p.q_start = q_start;
+    p.part = reinterpret_cast<float*>(workspace);
+    int* range = reinterpret_cast<int*>(reinterpret_cast<char*>(workspace) + n.part_bytes);
+    p.doc_range = range;
+    p.qb = strides[0]; p.qh = strides[1]; p.qs = strides[2];
+    p.kb = strides[3]; p.kh = strides[4]; p.ks = strides[5];
+    p.vb = strides[6]; p.vh = strides[7]; p.vs = strides[8];
+    p.ob = strides[9]; p.os = strides[10];
+    p.qd_ld = q_docs_ld; p.kd_ld = kv_docs_ld;
+    p.B = batch; p.Hq = q_heads; p.Hkv = kv_heads; p.Sq = q_len; p.Sk = kv_len; p.group = n.group; p.pack = n.pack;
+    p.causal = causal; p.reach = reach; p.splits = n.splits; p.row_tiles = n.row_tiles; p.key_tiles = n.key_tiles;
+    p.scale = scale; p.cap = cap;
+    hipStream_t st = (hipStream_t)stream;
+    if (n.range_bytes)
+        hipLaunchKernelGGL(doc_range_kernel, dim3((unsigned)n.key_tiles, (unsigned)batch), dim3(64), 0, st, kv_docs, range, kv_docs_ld, kv_len,
+                           n.key_tiles);
+    return head_dim == 128 ? dispatch_text<128>(p, n, st) : dispatch_text<64>(p, n, st);
+}

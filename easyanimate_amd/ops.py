@@ -682,6 +682,79 @@ def attention_causal_gqa(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, seq
     return out
 
 
+def _strided(t: torch.Tensor):
+    """(t, its batch / head / row strides) as ea_attention_text_bf16 reads them: unit inner stride, strides multiples of 8 (those of
+    one-element axes do not count), 16-byte aligned -- or a contiguous copy where t is not like that."""
+    st = [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s in st):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        st = [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
+    return t, st
+
+
+def attention_text(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *, causal: bool = False, cap: float = 0.0,
+                   bias: Optional[torch.Tensor] = None, q_docs: Optional[torch.Tensor] = None, kv_docs: Optional[torch.Tensor] = None,
+                   prefix: Optional[torch.Tensor] = None, valid: Optional[torch.Tensor] = None, q_start: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(f(q k^T scale)) v of text models: q bf16 [B, Hq, Sq, D], k / v bf16 [B, Hkv, Sk, D] (D 64 or 128, strides free: views of
+    projection outputs or a cache), head h reads kv head h // (Hq // Hkv) -> bf16 [B, Sq, Hq * D].
+      cap > 0      scores become cap * tanh(score / cap)
+      bias         fp32 [Hq, 2 R + 1]: bias[h, clamp(j - p, -R, R) + R] is added for key j and query position p
+      causal       key j <= p only; prefix int32 [B]: and the keys below prefix[b], seen by every query
+      q_docs / kv_docs   int32 [B, Sq] / [B, Sk]: only keys of the query's document (ids arbitrary; packed documents are skipped fast)
+      valid        int32 [B]: keys that exist
+      q_start      int32 [B]: position of the first query (default Sk - Sq: the queries are the last tokens)
+    A query that sees no key gives zeros.  One new token against a long cache is split over the GPU.  (ea_attention_text_bf16)"""
+    _chk(q, _BF16, "q"); _chk(k, _BF16, "k"); _chk(v, _BF16, "v")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"q, k, v: expected [B, H, S, D] with k and v alike, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, Hq, Sq, D = q.shape
+    Hkv, Sk = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not belong together (batch, head_dim, heads a multiple of kv heads)")
+    if D not in (64, 128):
+        raise ValueError(f"head_dim {D}: 64 and 128 are built")
+    if not (0.0 < scale < float("inf")) or not (0.0 <= cap < float("inf")):
+        raise ValueError(f"scale must be positive and finite, cap positive and finite or 0 (got {scale}, {cap})")
+    reach = 0
+    if bias is not None:
+        _chk(bias, _F32, "bias")
+        if bias.dim() != 2 or bias.shape[0] != Hq or bias.shape[1] % 2 != 1 or not bias.is_contiguous():
+            raise ValueError(f"bias: expected contiguous [{Hq}, 2 R + 1], got {tuple(bias.shape)}")
+        reach = bias.shape[1] // 2
+    if (q_docs is None) != (kv_docs is None):
+        raise ValueError("q_docs and kv_docs come together")
+    if prefix is not None and not causal:
+        raise ValueError("prefix needs causal order")
+    for t, name, shape in ((q_docs, "q_docs", (B, Sq)), (kv_docs, "kv_docs", (B, Sk)), (prefix, "prefix", (B,)), (valid, "valid", (B,)),
+                           (q_start, "q_start", (B,))):
+        if t is not None:
+            _chk(t, torch.int32, name)
+            if t.shape != shape or (t.shape[-1] > 1 and t.stride(-1) != 1):
+                raise ValueError(f"{name}: expected {shape} with unit inner stride, got {tuple(t.shape)}, strides {t.stride()}")
+    with _same_device(q.device, k, v, bias, q_docs, kv_docs, prefix, valid, q_start, out):
+        if out is None:
+            out = torch.empty((B, Sq, Hq * D), dtype=_BF16, device=q.device)
+        _chk(out, _BF16, "out")
+        if out.shape != (B, Sq, Hq * D) or out.stride(2) != 1:
+            raise ValueError(f"out: expected [{B}, {Sq}, {Hq * D}] with unit inner stride, got {tuple(out.shape)}, strides {out.stride()}")
+        if B == 0 or Sq == 0:
+            return out
+        if Sk == 0:
+            return out.zero_()
+        (q, sq), (k, sk), (v, sv) = _strided(q), _strided(k), _strided(v)
+        strides = (ctypes.c_int64 * 11)(*sq, *sk, *sv, out.stride(0) if B > 1 else 0, out.stride(1) if Sq > 1 else 0)
+        need = _lib.load().ea_attention_text_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, int(q_docs is not None))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _timed("attention", lambda: _lib.call("ea_attention_text_bf16", _p(q), _p(k), _p(v), _p(out), ctypes.addressof(strides), B, Hq, Hkv, Sq, Sk,
+                                              D, float(scale), int(causal), float(cap), _p(bias), reach, _p(q_docs), _p(kv_docs),
+                                              q_docs.stride(0) if q_docs is not None else 0, kv_docs.stride(0) if kv_docs is not None else 0,
+                                              _p(prefix), _p(valid), _p(q_start), _p(ws), need, _stream()))
+    return out
+
+
 def tile_blend_(a: torch.Tensor, b: torch.Tensor, extent: int, axis: int) -> torch.Tensor:
     """In place on b: the seam blend of two neighbouring VAE tiles [B,C,T,H,W] (contiguous, same dtype bf16 / fp32), axis 3 =
     blend_v (a above b), axis 4 = blend_h (a left of b); autoencoder_magvit.py:319-337."""

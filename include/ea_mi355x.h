@@ -405,6 +405,27 @@ int ea_silu_mul_bf16(const ea_bf16* gate, const ea_bf16* up, ea_bf16* out, int64
 int ea_attention_causal_gqa_bf16(const ea_bf16* q, const ea_bf16* k, const ea_bf16* vt, ea_bf16* out, const int* valid, int batch,
                                  int q_heads, int kv_heads, int seq, int s_pad, int head_dim, int causal, float scale, void* stream);
 
+/* Attention of text models in general, grouped-query heads, any lengths (one new token against a cache included):
+ *     t = scale q.k;  cap > 0: t = cap tanh(t / cap);  bias: t += bias[h][clamp(j - p, -reach, reach) + reach]
+ *     out = softmax over the visible keys of t, times v;     p = q_start[b] + i is the position of query i (NULL: kv_len - q_len + i)
+ * Key j is visible to query i of batch element b when  j < valid[b]  (valid NULL: kv_len)  and  (causal == 0 or j <= p or
+ * j < prefix[b])  and  kv_docs[b][j] == q_docs[b][i]  (both NULL: no documents; ids are arbitrary, cheapest where equal ids are
+ * neighbours).  A query that sees no key, or only scores of -inf, gives zeros; values and scores of hidden keys do not reach the
+ * result whatever they are (a key hidden from one query may hold a NaN that another query sees).
+ *   q bf16 [batch, q_heads, q_len, D], k / v bf16 [batch, kv_heads, kv_len, D]: any batch, head and row strides; out bf16
+ *   [batch, q_len, q_heads * D] by batch and row stride.  strides: HOST array of 11 element strides -- q batch, head, row; k ..;
+ *   v ..; out batch, row -- non-negative multiples of 8; pointers 16-byte aligned.  D = 64 or 128; head h reads kv head
+ *   h / (q_heads / kv_heads).  bias fp32 [q_heads][2 reach + 1] or NULL (lowest-float entries keep their order, -inf hides);
+ *   q_docs / kv_docs int32 with row strides q_docs_ld / kv_docs_ld; prefix, valid, q_start int32 [batch] or NULL (prefix: causal only).
+ * scale > 0.  workspace: ea_attention_text_workspace_bytes() bytes of the caller's (documents = 1 when q_docs is given), 0 for many
+ * shapes; calls that may run at the same time need one each.  Results do not depend on timing. */
+int64_t ea_attention_text_workspace_bytes(int batch, int q_heads, int kv_heads, int q_len, int kv_len, int head_dim, int documents);
+int ea_attention_text_bf16(const ea_bf16* q, const ea_bf16* k, const ea_bf16* v, ea_bf16* out, const int64_t* strides, int batch,
+                           int q_heads, int kv_heads, int q_len, int kv_len, int head_dim, float scale, int causal, float cap,
+                           const float* bias, int reach, const int* q_docs, const int* kv_docs, int64_t q_docs_ld, int64_t kv_docs_ld,
+                           const int* prefix, const int* valid, const int* q_start, void* workspace, int64_t workspace_bytes,
+                           void* stream);
+
 /* Spatial tiling of the VAE wrapper (use_tiling / use_tiling_encoder / use_tiling_decoder, autoencoder_magvit.py:249-254,276-279):
  * the seam blends of tiled_encode / tiled_decode, blend_v (:319-327) and blend_h (:329-337), in place on tile b:
  *     b[o, y, i] = a[o, a_n - extent + y, i] * (1 - y / extent) + b[o, y, i] * (y / extent)      y < extent, i < inner, o < outer
