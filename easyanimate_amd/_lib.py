@@ -33,7 +33,7 @@ PROTOTYPES = {
     "ea_gemm_bf16_w8": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _L, _L, _L, _L, _L, _L, _L, _I, _P],
     "ea_mxfp4_quantize_bf16": [_P, _P, _P, _L, _I, _L, _P],
     "ea_mxfp4_dequantize_bf16": [_P, _P, _P, _L, _I, _P],
-    "ea_gemm_mxfp4_workspace_bytes": [_I, _I, _I, _I],
+    "ea_gemm_mxfp4_workspace_bytes": [_I, _I, _I, _I, _I],
     "ea_gemm_mxfp4": [_P] * 9 + [_I, _I, _I, _I, _L, _L, _L, _L, _L, _L, _L, _I, _P, _L, _P],
     "ea_qknorm_rope_bf16": [_P, _L, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F, _P],
     "ea_qkv_gemm_norm_rope_bf16": [_P] * 16 + [_I, _I, _I, _I, _L, _L, _I, _I, _I, _I, _I, _F, _F, _P],

@@ -56,12 +56,11 @@ __device__ __forceinline__ void glds16t(const void* gptr, void* lds_wave_base) {
                                      (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
 }
 
-// 16-byte-chunk swizzles of the LDS rows (2 D bytes each).  K fragments read rows {0..3, 8..11, ..} of a block eight lanes at a time:
-// all different in the low three bits.  V's transposed reads take 32-byte pieces of rows {0..3} of every 8: the piece index moves.
+// 16-byte-chunk swizzle of the LDS rows (2 D bytes each), the same for K and V: an even number, so that 32-byte pairs of chunks stay
+// together.  K fragments: eight lanes read rows {0..3, 8..11} at one chunk and eight others the neighbouring chunk; V's transposed
+// reads: 32-byte pieces of rows {0..3} of every eight.  Either way the pieces land in different banks.
 template <int D>
-__device__ __forceinline__ int k_swz(int row) { return (row & 3) | ((row >> 3) & 1) << 2; }
-template <int D>
-__device__ __forceinline__ int v_swz(int row) {
+__device__ __forceinline__ int swz(int row) {
     return D == 128 ? 2 * ((row & 3) | ((row >> 3) & 1) << 2) : 2 * (((row >> 1) & 1) | ((row >> 3) & 1) << 1);
 }
 
@@ -242,7 +241,7 @@ __device__ __forceinline__ void block_step(const TextArgs& p, Rows<D, RT>& R, co
     const int vrow = 8 * lq + (lr >> 2);
 #pragma unroll
     for (int d = 0; d < NT; ++d) {
-        const int ch = ((2 * d + ((lr & 3) >> 1)) ^ v_swz<D>(vrow)) * 16 + (lr & 1) * 8;     // (+ 4 rows: the same swizzle)
+        const int ch = ((2 * d + ((lr & 3) >> 1)) ^ swz<D>(vrow)) * 16 + (lr & 1) * 8;     // (+ 4 rows: the same swizzle)
         const char* a = vtile + vrow * (2 * D) + ch;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 4 * (2 * D)));
@@ -272,7 +271,7 @@ __device__ __forceinline__ void block_step(const TextArgs& p, Rows<D, RT>& R, co
                         for (int r = 0; r < 4; ++r) {
                             const int col = 16 * d + lq * 4 + r;
                             const unsigned short bits = *reinterpret_cast<const unsigned short*>(
-                                vtile + key * (2 * D) + (((col >> 3) ^ v_swz<D>(key)) << 4) + (col & 7) * 2);
+                                vtile + key * (2 * D) + (((col >> 3) ^ swz<D>(key)) << 4) + (col & 7) * 2);
                             if (seen && (bits & 0x7f80) == 0x7f80) R.o[t][d][r] += bf16_bits_to_f32(bits);
                         }
                     }
@@ -410,8 +409,8 @@ __global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
             const int r = (wave * PIECES + i) * PER + lane / (D / 8), cs = lane % (D / 8);
             int key = t * TKEYS + r;
             key = key < p.Sk ? key : p.Sk - 1;
-            glds16t(Kh + (int64_t)key * p.ks + ((cs ^ k_swz<D>(r)) << 3), ks + i * 1024);
-            glds16t(Vh + (int64_t)key * p.vs + ((cs ^ v_swz<D>(r)) << 3), ks + OPER + i * 1024);
+            glds16t(Kh + (int64_t)key * p.ks + ((cs ^ swz<D>(r)) << 3), ks + i * 1024);
+            glds16t(Vh + (int64_t)key * p.vs + ((cs ^ swz<D>(r)) << 3), ks + OPER + i * 1024);
         }
     };
     // bias window of tile t: entry w of head g = bias at distance 64 t - position(q_last) + w, in the log2 domain.  Finite values stay
@@ -459,7 +458,7 @@ __global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
                     const int row = blk * 32 + 8 * (lr >> 2) + 4 * kt + (lr & 3);
 #pragma unroll
                     for (int s = 0; s < D / 32; ++s)
-                        kf[kt][s] = *reinterpret_cast<const bf16x8*>(kt0 + row * (2 * D) + (((s * 4 + lq) ^ k_swz<D>(row)) << 4));
+                        kf[kt][s] = *reinterpret_cast<const bf16x8*>(kt0 + row * (2 * D) + (((s * 4 + lq) ^ swz<D>(row)) << 4));
                 }
                 int docs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
                 if (masked && p.q_docs) {
@@ -525,7 +524,7 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
             const int r = i * PER + lane / (D / 8), cs = lane % (D / 8);
             int key = blk * 32 + r;
             key = key < p.Sk ? key : p.Sk - 1;
-            glds16t(Vh + (int64_t)key * p.vs + ((cs ^ v_swz<D>(r)) << 3), mine + stage * OPER + i * 1024);
+            glds16t(Vh + (int64_t)key * p.vs + ((cs ^ swz<D>(r)) << 3), mine + stage * OPER + i * 1024);
         }
     };
     bf16x8 kf[2][D / 32];

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-from typing import NamedTuple, Optional, Union
+from typing import Optional, Union
 
 import torch
 
@@ -243,15 +243,6 @@ def gemm_kblocked(A: torch.Tensor, W: torch.Tensor, bias: Optional[torch.Tensor]
 
 
 # ---- microscaled 4-bit storage --------------------------------------------------------------------
-class Mxfp4(NamedTuple):
-    """A [rows, k] matrix in microscaled 4-bit storage (mxfp4_quantize): codes uint8 [ceil(k/256), rows, 128] (two e2m1 codes a byte,
-    low nibble first), scales uint8 [ceil(k/256), rows, 8] (2^(byte - 127) per block of 32 elements of a row; 255 = NaN)."""
-    codes: torch.Tensor
-    scales: torch.Tensor
-    rows: int
-    k: int
-
-
 _NO_GUARD = contextlib.nullcontext()
 
 
@@ -264,17 +255,44 @@ def _same_device(dev: torch.device, *ts):
             raise RuntimeError(f"easyanimate_amd.ops: tensors on different devices ({dev} and {t.device})")
     if dev.type != "cuda":
         raise RuntimeError("easyanimate_amd.ops: tensors must live on the GPU -- the hot path has no CPU fallback")
-    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _NO_GUARD if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
-def _chk_mxfp4(t: Mxfp4, name: str):
-    kt = (t.k + 255) // 256
-    if t.codes.dtype != torch.uint8 or t.scales.dtype != torch.uint8:
-        raise TypeError(f"{name}: codes and scales must be uint8")
-    if t.k < 1 or t.codes.shape != (kt, t.rows, 128) or t.scales.shape != (kt, t.rows, 8):
-        raise ValueError(f"{name}: codes {tuple(t.codes.shape)} / scales {tuple(t.scales.shape)} are not those of a [{t.rows}, {t.k}] matrix")
-    if not (t.codes.is_contiguous() and t.scales.is_contiguous()):
-        raise ValueError(f"{name}: codes and scales must be contiguous")
+def _a(t: Optional[torch.Tensor]):
+    """Address for a c_void_p argument (an int: ctypes wraps it)."""
+    return None if t is None else t.data_ptr()
+
+
+def _stream_on(dev: torch.device) -> int:
+    """The current stream of `dev` as an address (torch.cuda.current_stream() costs more than a small kernel's launch)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+class Mxfp4:
+    """A [rows, k] matrix in microscaled 4-bit storage (mxfp4_quantize): codes uint8 [ceil(k/256), rows, 128] (two e2m1 codes a byte,
+    low nibble first), scales uint8 [ceil(k/256), rows, 8] (2^(byte - 127) per block of 32 elements of a row, block 4 j + g of a tile
+    at byte 2 g + j; 255 = NaN).
+    Checked once, here; its fields are not to be re-bound."""
+    __slots__ = ("codes", "scales", "rows", "k")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, k: int):
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("Mxfp4: codes and scales must be uint8")
+        kt = (k + 255) // 256
+        if k < 1 or codes.shape != (kt, rows, 128) or scales.shape != (kt, rows, 8):
+            raise ValueError(f"Mxfp4: codes {tuple(codes.shape)} / scales {tuple(scales.shape)} are not those of a [{rows}, {k}] matrix")
+        if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() % 16 or scales.data_ptr() % 8:
+            raise ValueError("Mxfp4: codes and scales must be contiguous, codes 16-byte and scales 8-byte aligned")
+        if codes.device != scales.device:
+            raise RuntimeError(f"Mxfp4: codes on {codes.device}, scales on {scales.device}")
+        self.codes, self.scales, self.rows, self.k = codes, scales, rows, k
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def to(self, device) -> "Mxfp4":
+        return Mxfp4(self.codes.to(device), self.scales.to(device), self.rows, self.k)
 
 
 def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
@@ -283,22 +301,25 @@ def mxfp4_quantize(x: torch.Tensor) -> Mxfp4:
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x: expected [rows, k >= 1], got {tuple(x.shape)}")
     rows, k = x.shape
-    if rows > 1 and (x.stride(1) != 1 or x.stride(0) < k) or k > 1 and x.stride(1) != 1:
-        x = x.contiguous()
-    kt = (k + 255) // 256
-    with _same_device(x.device):
-        codes = torch.empty((kt, rows, 128), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((kt, rows, 8), dtype=torch.uint8, device=x.device)
-        _lib.call("ea_mxfp4_quantize_bf16", _p(x), _p(codes), _p(scales), rows, k, max(k, x.stride(0)), _stream())
-    return Mxfp4(codes, scales, rows, k)
+    ld = x.stride(0) if rows > 1 else k
+    if ld < k or (k > 1 and x.stride(1) != 1):
+        x, ld = x.contiguous(), k
+    kt, dev = (k + 255) // 256, x.device
+    q = object.__new__(Mxfp4)
+    with _same_device(dev):
+        q.codes = torch.empty((kt, rows, 128), dtype=torch.uint8, device=dev)
+        q.scales = torch.empty((kt, rows, 8), dtype=torch.uint8, device=dev)
+        q.rows, q.k = rows, k
+        _lib.call("ea_mxfp4_quantize_bf16", x.data_ptr(), q.codes.data_ptr(), q.scales.data_ptr(), rows, k, ld, _stream_on(dev))
+    return q
 
 
 def mxfp4_dequantize(q: Mxfp4) -> torch.Tensor:
     """The bf16 [rows, k] values that q stands for (exact)."""
-    _chk_mxfp4(q, "q")
-    with _same_device(q.codes.device, q.scales):
-        y = torch.empty((q.rows, q.k), dtype=_BF16, device=q.codes.device)
-        _lib.call("ea_mxfp4_dequantize_bf16", _p(q.codes), _p(q.scales), _p(y), q.rows, q.k, _stream())
+    dev = q.codes.device
+    with _same_device(dev):
+        y = torch.empty((q.rows, q.k), dtype=_BF16, device=dev)
+        _lib.call("ea_mxfp4_dequantize_bf16", q.codes.data_ptr(), q.scales.data_ptr(), y.data_ptr(), q.rows, q.k, _stream_on(dev))
     return y
 
 
@@ -307,61 +328,63 @@ def gemm_mxfp4(A: Union[torch.Tensor, Mxfp4], W: Mxfp4, bias: Optional[torch.Ten
     """out[b] = epi(A[b] @ W.T + bias) over 4-bit operands, W of a [N, K] nn.Linear weight (N % 8 == 0).  A: bf16 [B, M, K] or [M, K]
     (quantised here: mxfp4_quantize's values), or the Mxfp4 of [M, K].  bias fp32 [N]; out bf16 [B, M, N] (fp32 for EPI_F32_OUT); res
     bf16 like out (may alias out); gate fp32 [B, N] ([N] for two-dimensional A); epilogues as gemm()."""
-    _chk_mxfp4(W, "W")
+    if not isinstance(W, Mxfp4):
+        raise TypeError(f"W: expected Mxfp4, got {type(W).__name__}")
     N, K = W.rows, W.k
     packed = isinstance(A, Mxfp4)
+    lda = abs_ = 0
     if packed:
-        _chk_mxfp4(A, "A")
         B, M, ak, squeeze, dev = 1, A.rows, A.k, True, A.codes.device
     else:
         _chk(A, _BF16, "A")
-        if A.dim() not in (2, 3):
-            raise ValueError(f"A: expected [M, K] or [B, M, K], got {tuple(A.shape)}")
         squeeze, dev = A.dim() == 2, A.device
         if squeeze:
-            A = A.unsqueeze(0)
-        B, M, ak = A.shape
+            B, (M, ak) = 1, A.shape
+        elif A.dim() == 3:
+            B, M, ak = A.shape
+        else:
+            raise ValueError(f"A: expected [M, K] or [B, M, K], got {tuple(A.shape)}")
+        if ak > 1 and A.stride(-1) != 1:
+            A = A.contiguous()
+        lda = A.stride(-2) if M > 1 else 0
+        abs_ = A.stride(0) if B > 1 else 0
     if ak != K:
         raise ValueError(f"A has K = {ak}, W has K = {K}")
     if epilogue not in (EPI_BIAS, EPI_BIAS_GELU_TANH, EPI_BIAS_GATE_RES, EPI_F32_OUT):
         raise ValueError(f"unknown epilogue {epilogue}")
-    if squeeze:
-        out = out.unsqueeze(0) if out is not None else None
-        res = res.unsqueeze(0) if res is not None else None
-        gate = gate.unsqueeze(0) if gate is not None and gate.dim() == 1 else gate
     odt = _F32 if epilogue == EPI_F32_OUT else _BF16
-    with _same_device(dev, W.codes, W.scales, bias, out, res, gate, A.scales if packed else None):
+    shape = (M, N) if squeeze else (B, M, N)
+    with _same_device(dev, W.codes, bias, out, res, gate):
         if out is None:
-            out = torch.empty((B, M, N), dtype=odt, device=dev)
-        _chk(out, odt, "out")
-        if out.shape != (B, M, N) or out.stride(2) != 1:
-            raise ValueError(f"out: expected [{B}, {M}, {N}] with unit inner stride, got {tuple(out.shape)}, strides {out.stride()}")
+            out = torch.empty(shape, dtype=odt, device=dev)
+            ldc, cbs = N, M * N
+        else:
+            _chk(out, odt, "out")
+            if out.shape != shape or out.stride(-1) != 1:
+                raise ValueError(f"out: expected {list(shape)} with unit inner stride, got {tuple(out.shape)}, strides {out.stride()}")
+            ldc, cbs = (out.stride(-2) if M > 1 else N), (out.stride(0) if B > 1 else 0)
         if bias is not None:
             _chk(bias, _F32, "bias")
-            if bias.shape != (N,) or not bias.is_contiguous():
+            if bias.shape != (N,) or (N > 1 and bias.stride(0) != 1):
                 raise ValueError(f"bias: expected contiguous [{N}], got {tuple(bias.shape)}")
         ldres = rbs = gbs = 0
         if epilogue == EPI_BIAS_GATE_RES:
             if res is None or gate is None:
                 raise ValueError("EPI_BIAS_GATE_RES needs res and gate")
             _chk(res, _BF16, "res"); _chk(gate, _F32, "gate")
-            if res.shape != (B, M, N) or res.stride(2) != 1 or gate.shape != (B, N) or gate.stride(1) != 1:
-                raise ValueError(f"res / gate: expected [{B}, {M}, {N}] / [{B}, {N}] with unit inner stride, got {tuple(res.shape)} / {tuple(gate.shape)}")
-            ldres, rbs, gbs = res.stride(1), res.stride(0), gate.stride(0)
-        if B * M:
-            x, lda, abs_ = None, 0, 0
-            if not packed:
-                # few rows: the product quantises them itself (one launch); else once, in front of it
-                if M <= 16 and K % 8 == 0 and A.stride(2) == 1 and A.stride(1) % 8 == 0 and A.stride(0) % 8 == 0 and A.data_ptr() % 16 == 0:
-                    x, lda, abs_ = A, A.stride(1), A.stride(0)
-                else:
-                    A = mxfp4_quantize(A.reshape(B * M, K))
-            need = _lib.load().ea_gemm_mxfp4_workspace_bytes(B, M, N, K)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _timed("gemm", lambda: _lib.call("ea_gemm_mxfp4", None if x is not None else _p(A.codes), None if x is not None else _p(A.scales), _p(x),
-                                             _p(W.codes), _p(W.scales), _p(bias), _p(out), _p(res), _p(gate), B, M, N, K, lda, abs_,
-                                             out.stride(1), out.stride(0), ldres, rbs, gbs, int(epilogue), _p(ws), need, _stream()))
-    return out.squeeze(0) if squeeze else out
+            if squeeze and gate.dim() == 1:
+                gate = gate.unsqueeze(0)
+            if res.shape != shape or res.stride(-1) != 1 or gate.shape != (B, N) or gate.stride(1) != 1:
+                raise ValueError(f"res / gate: expected {list(shape)} / [{B}, {N}] with unit inner stride, got {tuple(res.shape)} / {tuple(gate.shape)}")
+            ldres, rbs, gbs = (res.stride(-2) if M > 1 else 0), (res.stride(0) if B > 1 else 0), (gate.stride(0) if B > 1 else 0)
+        if B * M == 0:
+            return out
+        need = _lib.load().ea_gemm_mxfp4_workspace_bytes(B, M, N, K, not packed)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        qa, sa, x = (A.codes.data_ptr(), A.scales.data_ptr(), None) if packed else (None, None, A.data_ptr())
+        _timed("gemm", lambda: _lib.call("ea_gemm_mxfp4", qa, sa, x, W.codes.data_ptr(), W.scales.data_ptr(), _a(bias), out.data_ptr(), _a(res), _a(gate),
+                                         B, M, N, K, lda, abs_, ldc, cbs, ldres, rbs, gbs, epilogue, _a(ws), need, _stream_on(dev)))
+    return out
 
 
 # Softmax scale of head_dim 64 folded into Q (exp2 domain): q_scale = 64^-1/2 * log2(e) at ea_qknorm_rope_bf16, and
@@ -685,13 +708,14 @@ def attention_causal_gqa(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, seq
 def _strided(t: torch.Tensor):
     """(t, its batch / head / row strides) as ea_attention_text_bf16 reads them: unit inner stride, strides multiples of 8 (those of
     one-element axes do not count), 16-byte aligned -- or a contiguous copy where t is not like that."""
-    st = [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s in st):
+    sh, (b, h, s, d) = t.shape, t.stride()
+    b, h, s = b if sh[0] > 1 else 0, h if sh[1] > 1 else 0, s if sh[2] > 1 else 0
+    if d != 1 or (b | h | s) & 7 or t.data_ptr() & 15:
         t = t.contiguous()
-        if t.data_ptr() % 16:
+        if t.data_ptr() & 15:
             t = t.clone()
-        st = [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
-    return t, st
+        return t, (t.stride(0), t.stride(1), t.stride(2))
+    return t, (b, h, s)
 
 
 def attention_text(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *, causal: bool = False, cap: float = 0.0,
@@ -748,10 +772,11 @@ def attention_text(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
         strides = (ctypes.c_int64 * 11)(*sq, *sk, *sv, out.stride(0) if B > 1 else 0, out.stride(1) if Sq > 1 else 0)
         need = _lib.load().ea_attention_text_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, int(q_docs is not None))
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        _timed("attention", lambda: _lib.call("ea_attention_text_bf16", _p(q), _p(k), _p(v), _p(out), ctypes.addressof(strides), B, Hq, Hkv, Sq, Sk,
-                                              D, float(scale), int(causal), float(cap), _p(bias), reach, _p(q_docs), _p(kv_docs),
-                                              q_docs.stride(0) if q_docs is not None else 0, kv_docs.stride(0) if kv_docs is not None else 0,
-                                              _p(prefix), _p(valid), _p(q_start), _p(ws), need, _stream()))
+        _timed("attention", lambda: _lib.call("ea_attention_text_bf16", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                              ctypes.addressof(strides), B, Hq, Hkv, Sq, Sk, D, scale, causal, cap, _a(bias), reach, _a(q_docs),
+                                              _a(kv_docs), q_docs.stride(0) if q_docs is not None else 0,
+                                              kv_docs.stride(0) if kv_docs is not None else 0, _a(prefix), _a(valid), _a(q_start), _a(ws), need,
+                                              _stream_on(q.device)))
     return out
 
 

@@ -144,8 +144,8 @@ int ea_gemm_bf16_w8(const ea_bf16* A, const uint8_t* W_fp8, const float* bias, e
 /* Blocks of 32 consecutive elements of a row share one scale 2^e, e = clamp(floor(log2 max|x|) - 2, -127, 127), stored as byte
  * e + 127; an element is the e2m1 code {0, 0.5, 1, 1.5, 2, 3, 4, 6} nearest to x / 2^e (ties to the even code, 6 at most) with its
  * sign.  A block holding an infinity or a NaN is byte 255 (NaN) with codes 0; a block of zeros byte 0.
- * Layout, K-blocked: codes [ceil(K/256)][rows][128] bytes (low nibble first), scales [ceil(K/256)][rows][8] bytes; the elements
- * past K of the last tile are zeros.  x: bf16 [rows, K], row stride ld >= K elements; K and ld need no alignment (multiples of 8 on
+ * Layout, K-blocked: codes [ceil(K/256)][rows][128] bytes (low nibble first), scales [ceil(K/256)][rows][8] bytes with the scale of
+ * the tile's block 4 j + g (j < 2, g < 4) at byte 2 g + j; the elements past K of the last tile are zeros.  x: bf16 [rows, K], row stride ld >= K elements; K and ld need no alignment (multiples of 8 on
  * 16-byte aligned rows are read in 16-byte pieces).  codes 16-byte, scales 8-byte aligned.  Every byte of both outputs is written. */
 int ea_mxfp4_quantize_bf16(const ea_bf16* x, uint8_t* codes, uint8_t* scales, int64_t rows, int K, int64_t ld, void* stream);
 
@@ -155,12 +155,13 @@ int ea_mxfp4_dequantize_bf16(const uint8_t* codes, const uint8_t* scales, ea_bf1
 /* for b in [0, batch): C_b[M, N] = epi(A_b . W^T + bias) over the STORED values of A and W, fp32 accumulation; epilogues as
  * ea_gemm_bf16 (EA_EPI_F32_OUT: C, ldc and c_batch_stride in floats).  W: codes / scales of [N, K].  The activations are either
  *   A / A_scales of [batch * M, K] (element b = rows [b M, (b + 1) M)), A_bf16 NULL, or
- *   A_bf16 [batch][M][lda] with M <= 16 and K, lda, a_batch_stride multiples of 8: quantised on the way, same codes, same result.
+ *   A_bf16 [batch][M][lda] (any strides), A and A_scales NULL: quantised on the way or into the workspace -- same codes, same result.
  * C bf16 (fp32) row stride ldc; res as ea_gemm_bf16 (may alias C); gate fp32 [batch][gate_batch_stride].
  * N, ldc, ldres and the batch strides of C and res % 8 == 0, gate_batch_stride % 4 == 0, pointers 16-byte (scales 8-byte) aligned.
- * workspace: ea_gemm_mxfp4_workspace_bytes() bytes of the caller's, 0 for many shapes (fp32 partial products of a K split, summed in
- * a fixed order: results do not depend on timing); calls that may run at the same time need one each. */
-int64_t ea_gemm_mxfp4_workspace_bytes(int batch, int M, int N, int K);
+ * workspace: ea_gemm_mxfp4_workspace_bytes() bytes of the caller's (a_is_bf16 = 1 when A_bf16 is given), 0 for many shapes: stored
+ * activations, and fp32 partial products of a K split, summed in a fixed order (results do not depend on timing).  Calls that may
+ * run at the same time need one each. */
+int64_t ea_gemm_mxfp4_workspace_bytes(int batch, int M, int N, int K, int a_is_bf16);
 int ea_gemm_mxfp4(const uint8_t* A, const uint8_t* A_scales, const ea_bf16* A_bf16, const uint8_t* W, const uint8_t* W_scales,
                   const float* bias, void* C, const ea_bf16* res, const float* gate, int batch, int M, int N, int K, int64_t lda,
                   int64_t a_batch_stride, int64_t ldc, int64_t c_batch_stride, int64_t ldres, int64_t res_batch_stride,

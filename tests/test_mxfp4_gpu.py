@@ -44,7 +44,9 @@ def values(codes, byte):
 def unpack(q):
     """ops.Mxfp4 -> (codes [rows, kp], bytes [rows, kp / 32]) on the host."""
     c = q.codes.cpu().permute(1, 0, 2).reshape(q.rows, -1)
-    return torch.stack([c & 15, c >> 4], -1).view(q.rows, -1), q.scales.cpu().permute(1, 0, 2).reshape(q.rows, -1)
+    kt = q.codes.shape[0]
+    s = q.scales.cpu().permute(1, 0, 2).reshape(q.rows, kt, 4, 2).transpose(2, 3)        # block 4 j + g at byte 2 g + j
+    return torch.stack([c & 15, c >> 4], -1).view(q.rows, kt * 256), s.reshape(q.rows, kt * 8)
 
 
 def _same_storage(x):
@@ -200,8 +202,11 @@ def test_product(M, N, K, epi):
     _run(x, w, N, epi, g)
 
 
-@pytest.mark.parametrize("M,N,K,kern", [(1, 64, 512, "gemm_mxfp4_skinny_bf16"), (1, 64, 513, "gemm_mxfp4_skinny"), (33, 64, 512, "gemm_mxfp4_skinny"),
-                                        (100, 256, 8192, "gemm_mxfp4_128_split"), (2200, 2048, 520, "gemm_mxfp4_128")])
+@pytest.mark.parametrize("M,N,K,kern", [(1, 64, 512, "gemm_mxfp4_skinny_bf16"), (1, 64, 513, "gemm_mxfp4_skinny"), (32, 64, 512, "gemm_mxfp4_skinny"),
+                                        (33, 64, 512, "gemm_mxfp4_64x64"), (20, 8200, 300, "gemm_mxfp4_64x64"),
+                                        (300, 392, 40, "gemm_mxfp4_64x64"), (70, 136, 13000, "gemm_mxfp4_64x64_split"),
+                                        (500, 3200, 1100, "gemm_mxfp4_128x64"), (900, 4000, 700, "gemm_mxfp4_128x128"), (1900, 4072, 264, "gemm_mxfp4_256x128"),
+                                        (257, 16000, 520, "gemm_mxfp4_256x128")])
 def test_product_variants(M, N, K, kern):
     x, w, g = _operands(M, N, K, M + K)
     _run(x, w, N, "bias", g, kern=kern)
@@ -270,7 +275,7 @@ def test_no_rows_no_launch():
     assert ops.gemm_mxfp4(torch.empty(0, 64, dtype=torch.bfloat16, device=DEV), W, None).shape == (0, 16)
 
 
-@pytest.mark.parametrize("M,K", [(1, 512), (100, 8192)])
+@pytest.mark.parametrize("M,K", [(1, 512), (100, 13000)])
 def test_side_stream_and_graph(M, K):
     """On a stream of its own, and captured: replayed with new inputs between eager calls, every replay equals the eager result."""
     from easyanimate_amd import ops
