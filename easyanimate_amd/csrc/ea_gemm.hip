@@ -982,6 +982,8 @@ __global__ __launch_bounds__(256) void gemm256_w4a_kernel(GemmArgs p) {
 #endif
 }
 
+#include "ea_gemm_mxfp4_w4.inc"
+
 // =================================================================================================
 // Fused QKV projection: ONE launch computes q, k, v = Linear_{q,k,v}(x) for a token stream and finishes each
 // (128 tokens x one head) wave tile in its epilogue -- bias, qk-LayerNorm(64), interleaved RoPE, softmax scale on q,
@@ -1447,6 +1449,35 @@ int gemm_entry(const ea_bf16* A, const void* W, const float* bias, ea_bf16* C, c
 }
 
 }  // namespace
+
+// ea_gemm_mxfp4.hip's large products (gemm256_mxfp4_w4_kernel): codes / scales of [batch * M, K] and [N, K], kt K tiles; as_bytes = size of
+// the activation scales' buffer.  EA_ERR_ARG if an operand does not fit the kernel's 32-bit buffer offsets.
+int ea_gemm_mxfp4_w4_launch(const unsigned char* A, const unsigned char* As, int64_t as_bytes, const unsigned char* W, const unsigned char* Ws,
+                            const float* bias, void* C, const ea_bf16* res, const float* gate, int batch, int M, int N, int kt, int64_t ldc,
+                            int64_t cbs, int64_t ldres, int64_t rbs, int64_t gbs, int epilogue, hipStream_t st) {
+    const int64_t a_rows = (int64_t)batch * M, limit = 0xFFFFFFFFll;
+    if (a_rows * kt * 128 >= limit || (int64_t)N * kt * 128 >= limit || as_bytes >= limit || (int64_t)kt * 64 > 0x7fffffff) return EA_ERR_ARG;
+    GemmArgs p;
+    p.A = reinterpret_cast<const unsigned short*>(A); p.W = reinterpret_cast<const unsigned short*>(W); p.bias = bias;
+    p.C = reinterpret_cast<unsigned short*>(C); p.res = res; p.gate = gate;
+    p.M = M; p.N = N; p.K = kt * BK;
+    p.lda = 64; p.abs_ = (int64_t)M * 64; p.ldc = ldc; p.cbs = cbs; p.ldres = ldres; p.rbs = rbs; p.gbs = gbs;
+    p.a_kstep = a_rows * 64; p.w_kstep = (int64_t)N * 64; p.ldw = 64;
+    p.tiles_m = (M + 255) / 256;
+    p.tiles_n = (N + 255) / 256;
+    p.rows_per_xcd = p.tiles_m >= 64 ? (p.tiles_m + 7) / 8 : 0;
+    const dim3 grid(p.rows_per_xcd ? 8 * p.rows_per_xcd * p.tiles_n : p.tiles_m * p.tiles_n, batch);
+    const auto kern = epilogue == EA_EPI_BIAS ? gemm256_mxfp4_w4_kernel<EA_EPI_BIAS>
+                      : epilogue == EA_EPI_BIAS_GELU_TANH ? gemm256_mxfp4_w4_kernel<EA_EPI_BIAS_GELU_TANH> : gemm256_mxfp4_w4_kernel<EA_EPI_BIAS_GATE_RES>;
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, MXW4_LDS);
+    if (e != hipSuccess) {
+        ea_set_error("ea_gemm_mxfp4: %d bytes of LDS: %s", MXW4_LDS, hipGetErrorString(e));
+        return (int)e;
+    }
+    ea_count("gemm_mxfp4_256_w4");
+    hipLaunchKernelGGL(kern, grid, dim3(256), MXW4_LDS, st, p, As, Ws, as_bytes);
+    return EA_OK;
+}
 
 extern "C" int ea_gemm_bf16(const ea_bf16* A, const ea_bf16* W, const float* bias, ea_bf16* C,
                             const ea_bf16* res, const float* gate, int batch, int M, int N, int K, int64_t lda,

