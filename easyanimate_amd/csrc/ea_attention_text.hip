@@ -14,8 +14,8 @@
 // and, because K rows are fed in the order 8 (r / 4) + 4 kt + r % 4, eight consecutive keys of a 32-key block = its slice of the P^T
 // operand.  V stays row-major in memory and LDS; its transposed fragments come from ds_read_b64_tr_b16.  One pass with a running
 // maximum that is only moved when a score exceeds it by 2^8 (P then stays below 256 -- bf16 has fp32's exponent range -- and the
-// accumulators are hardly ever rescaled); P is rounded to bf16 for its product (2^-9 of each weight), the row sums are fp32 of the
-// unrounded weights.
+// accumulators are hardly ever rescaled); P is rounded to bf16 for its product (a relative half step of 2^-8 each); the row sums are
+// those of the rounded weights, by one more product with ones, in fp32.
 //
 //   attention_text_kernel       128 rows per workgroup (four waves, 32 rows each), K / V tiles of 64 keys double-buffered in LDS by
 //                               LDS-DMA; tiles that no row of the workgroup sees are skipped (64 at a time for documents)
@@ -49,11 +49,38 @@ struct TextArgs {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEG_INF = -__builtin_huge_valf();
-constexpr int BIAS_PACK_MAX = 16;       // heads packed into a row tile at most (bounds the bias window: see bias_window)
+constexpr int BIAS_PACK_MAX = 8;        // heads packed into a row tile at most (bounds the bias window: see bias_window)
 
-__device__ __forceinline__ void glds16t(const void* gptr, void* lds_wave_base) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)gptr,
-                                     (__attribute__((address_space(3))) void*)lds_wave_base, 16, 0, 0);
+// LDS-DMA requests, 16 (4) bytes per lane at byte offset voff of a resource of `extent` bytes; past its end zeros arrive.  Written in
+// assembly -- they have no result register -- because the compiler, where it sees them, waits for every request in flight in front of
+// each transposed LDS read.  (Its own counted waits stay right: requests that it does not count only make them wait longer.)
+typedef unsigned u32x4_s __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x4_s resource(const void* base, const unsigned extent) {
+    const uint64_t a = (uint64_t)(uintptr_t)base;
+    return u32x4_s{(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)a), (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)),
+                   (unsigned)__builtin_amdgcn_readfirstlane((int)extent), 0x00020000u};
+}
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+    return (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(size_t)(__attribute__((address_space(3))) const char*)p);
+}
+__device__ __forceinline__ void dma16(const u32x4_s rs, const int voff, const unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rs) : "m0", "memory");
+}
+// resource over `rows` rows of 2 D bytes, `step` elements apart (rows <= 0: empty)
+template <int D>
+__device__ __forceinline__ u32x4_s rows_resource(const unsigned short* from, const int step, const int rows) {
+    return resource(from, rows > 0 ? (unsigned)(rows - 1) * (unsigned)step * 2u + 2u * D : 0u);
+}
+__device__ __forceinline__ void words_to_lds(const int* from, const int words, const int voff, void* lds_wave_base) {
+    const u32x4_s rs = resource(from, words > 0 ? (unsigned)words * 4u : 0u);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds_address(lds_wave_base)), "v"(voff), "s"(rs)
+                 : "m0", "memory");
+}
+// the greater value, NaN where one is (no canonicalising moves in front of it, unlike fmaxf)
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float log2_bias(float v) {
+    const float big = 3.4028234663852886e38f;
+    return fabsf(v) <= big ? fminf(fmaxf(v * LOG2E, -big), big) : v;
 }
 
 // 16-byte-chunk swizzle of the LDS rows (2 D bytes each), the same for K and V: an even number, so that 32-byte pairs of chunks stay
@@ -68,13 +95,13 @@ __device__ __forceinline__ int swz(int row) {
 template <int D, int RT>
 struct Rows {
     bf16x8 q[RT][D / 32];
-    int64_t out_off[RT];      // element offset of the row's output, -1: no such row
     int lim[RT], doc[RT];     // keys below lim (and of the row's document) are visible
     int back[RT];             // distance bias: (last query of the tile) - (this query), + the row's head's window
     int lim_lo, lim_hi;       // over the wave's rows
     int doc_lo, doc_hi;
     f32x4 o[RT][D / 16];
-    float m[RT], l[RT];       // the reference maximum (log2 domain), this lane's share of the sum
+    float m[RT];              // the reference maximum (log2 domain)
+    f32x4 l[RT];              // the sum of the weights, in every element (a product with ones)
 };
 
 __device__ __forceinline__ int wave_min(int v) {
@@ -117,7 +144,6 @@ __device__ __forceinline__ void load_rows(const TextArgs& p, Rows<D, RT>& R, int
         const unsigned short* src = p.q + b * p.qb + (int64_t)(head0 + hg) * p.qh + (int64_t)qi * p.qs + lq * 8;
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) R.q[t][s] = *reinterpret_cast<const bf16x8*>(src + s * 32);
-        R.out_off[t] = live ? b * p.ob + (int64_t)qi * p.os + (int64_t)(head0 + hg) * D : -1;
         R.lim[t] = key_limit(p, b, qi);
         R.doc[t] = p.q_docs ? p.q_docs[b * p.qd_ld + qi] : 0;
         R.back[t] = hg * win + (qlast - qi);
@@ -126,7 +152,7 @@ __device__ __forceinline__ void load_rows(const TextArgs& p, Rows<D, RT>& R, int
         R.doc_lo = min(R.doc_lo, R.doc[t]);
         R.doc_hi = max(R.doc_hi, R.doc[t]);
         R.m[t] = NEG_INF;
-        R.l[t] = 0.f;
+        R.l[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) R.o[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -152,17 +178,39 @@ __device__ __forceinline__ float capped_log2(float s, float two_over, float c1, 
     return t;
 }
 
-// One 32-key block: scores of the wave's rows, softmax update, product with V.
-//   kf: its K fragments; vt: LDS byte address of this lane's transposed V reads (vtile + v_row_base); key0: its first key
-//   masked: some pair of the block may be hidden;  docs: this lane's 8 keys' documents (masked blocks of packed rows)
-//   win0: this lane's bias window position of key 8 lq of the block (bias variant)
-template <int D, int RT, bool CAP, bool BIAS>
-__device__ __forceinline__ void block_step(const TextArgs& p, Rows<D, RT>& R, const bf16x8 (&kf)[2][D / 32], const char* vtile, int key0, bool masked,
-                                           const int (&docs)[8], const float* win0, int lane) {
-    constexpr int NT = D / 16;
-    const int lr = lane & 15, lq = lane >> 4;
-    const float c = p.scale * LOG2E;
-    float s[RT][8];
+// K fragments of a 32-key block: A operand, key rows in the order 8 (r / 4) + 4 kt + r % 4.  V^T fragments: lane (lr, lq) of a transposed
+// read gets keys 8 lq + (0..3 | 4..7) of column 16 d + lr.  `at` is the block's LDS offset (a multiple of 256); a row's swizzle does not
+// reach the bits above the row, so a fragment's place is the lane's first one with the fragment's bits flipped.
+template <int D>
+__device__ __forceinline__ int k_lane(int lane) {
+    const int row = 8 * ((lane & 15) >> 2) + (lane & 3);
+    return row * (2 * D) + (((lane >> 4) ^ swz<D>(row)) << 4);
+}
+template <int D>
+__device__ __forceinline__ int v_lane(int lane) {
+    const int row = 8 * (lane >> 4) + ((lane & 15) >> 2);
+    return row * (2 * D) + ((((lane & 3) >> 1) ^ swz<D>(row)) << 4) + (lane & 1) * 8;
+}
+template <int D>
+__device__ __forceinline__ void read_k(const char* smem, int at, bf16x8 (&kf)[2][D / 32]) {       // at: + k_lane
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) kf[kt][s] = *reinterpret_cast<const bf16x8*>(smem + (at ^ (s * 64)) + kt * (8 * D));
+}
+template <int D>
+__device__ __forceinline__ void read_v(const char* smem, int at, u32x4_a (&vf)[D / 16]) {         // at: + v_lane
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+        const char* a = smem + (at ^ (d * 32));
+        const u32x2_a lo = __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a));
+        const u32x2_a hi = __builtin_bit_cast(u32x2_a, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 8 * D)));
+        vf[d] = u32x4_a{lo[0], lo[1], hi[0], hi[1]};
+    }
+}
+
+template <int D, int RT>
+__device__ __forceinline__ void block_qk(const Rows<D, RT>& R, const bf16x8 (&kf)[2][D / 32], float (&s)[RT][8]) {
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -173,41 +221,58 @@ __device__ __forceinline__ void block_step(const TextArgs& p, Rows<D, RT>& R, co
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[t][kt * 4 + r] = a[r];
         }
-    // ---- to the log2 domain where a cap or a bias makes the score more than a multiple of q.k; hidden pairs to -inf
-    float unit = c;                    // what a score still has to be multiplied with
+}
+
+// Scores -> weights of one 32-key block, state updated.  win0: this lane's bias window position of key 8 lq of the block.
+// masked: some pair of the block may be hidden; docs: this lane's 8 keys' documents (masked blocks of packed documents).
+template <int D, int RT, bool CAP, bool BIAS>
+__device__ __forceinline__ void block_softmax(const TextArgs& p, Rows<D, RT>& R, float (&s)[RT][8], bf16x8 (&pb)[RT], int key0, bool masked,
+                                              const int (&docs)[8], const float* win0, int lane) {
+    const int lq = lane >> 4;
+    const float c = p.scale * LOG2E;
+    // to the log2 domain where a cap or a bias makes the score more than a multiple of q.k
+    const float unit = CAP || BIAS ? 1.0f : c;                    // what a score still has to be multiplied with
     if (CAP) {
         const float c1 = p.cap * LOG2E, two_over = 2.0f * c / p.cap, half_over = p.scale / p.cap;
-        const bool wide = p.cap > 256.0f;
+        if (p.cap > 256.0f) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+            for (int t = 0; t < RT; ++t)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[t][e] = capped_log2(s[t][e], two_over, c1, half_over, wide);
-        unit = 1.0f;
+                for (int e = 0; e < 8; ++e) s[t][e] = capped_log2(s[t][e], two_over, c1, half_over, true);
+        } else {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[t][e] = capped_log2(s[t][e], two_over, c1, half_over, false);
+        }
     }
     if (BIAS) {
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[t][e] = __builtin_fmaf(s[t][e], unit, win0[R.back[t] + e]);
-        unit = 1.0f;
+            for (int e = 0; e < 8; ++e) s[t][e] = __builtin_fmaf(s[t][e], CAP ? 1.0f : c, win0[R.back[t] + e]);
     }
     if (masked) {
+        if (p.q_docs) {
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+            for (int t = 0; t < RT; ++t)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                bool see = key0 + 8 * lq + e < R.lim[t];
-                if (p.q_docs) see = see && docs[e] == R.doc[t];
-                s[t][e] = see ? s[t][e] : NEG_INF;
-            }
+                for (int e = 0; e < 8; ++e) s[t][e] = docs[e] == R.doc[t] ? s[t][e] : NEG_INF;
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            const int room = R.lim[t] - key0 - 8 * lq;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[t][e] = e < room ? s[t][e] : NEG_INF;
+        }
     }
-    // ---- move the reference maximum only when a row has outgrown it
+    // move the reference maximum only when a row has outgrown it
     float top[RT];
     bool grow = false;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        top[t] = fmaxf(fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])), fmaxf(fmaxf(s[t][4], s[t][5]), fmaxf(s[t][6], s[t][7]))) * unit;
-        grow = grow || top[t] > R.m[t] + 8.0f;
+        top[t] = max2(max2(max2(s[t][0], s[t][1]), max2(s[t][2], s[t][3])), max2(max2(s[t][4], s[t][5]), max2(s[t][6], s[t][7]))) * unit;
+        grow = grow | (top[t] > R.m[t] + 8.0f);
     }
     if (__ballot(grow)) {
 #pragma unroll
@@ -219,10 +284,9 @@ __device__ __forceinline__ void block_step(const TextArgs& p, Rows<D, RT>& R, co
             R.m[t] = n;
             R.l[t] *= alpha;
 #pragma unroll
-            for (int d = 0; d < NT; ++d) R.o[t][d] *= alpha;
+            for (int d = 0; d < D / 16; ++d) R.o[t][d] *= alpha;
         }
     }
-    bf16x8 pb[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const float ref = R.m[t] == NEG_INF ? 0.0f : R.m[t];
@@ -231,56 +295,76 @@ __device__ __forceinline__ void block_step(const TextArgs& p, Rows<D, RT>& R, co
         for (int e = 0; e < 8; e += 2) {
             const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], unit, -ref));
             const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e + 1], unit, -ref));
-            R.l[t] += p0 + p1;
             const f32x2 two = {p0, p1};
             pk[e >> 1] = __builtin_bit_cast(unsigned, __builtin_convertvector(two, bf16x2));
         }
         pb[t] = __builtin_bit_cast(bf16x8, pk);
     }
-    // ---- O^T += V^T P^T.  Lane (lr, lq) of a transposed read: keys 8 lq + (0..3 | 4..7), columns 16 d + lr.
-    const int vrow = 8 * lq + (lr >> 2);
+}
+
+// O^T += V^T P^T, and the sums of the same (rounded) weights
+template <int D, int RT>
+__device__ __forceinline__ void block_pv(Rows<D, RT>& R, const u32x4_a (&vf)[D / 16], const bf16x8 (&pb)[RT]) {
+    const u32x4_a ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
-    for (int d = 0; d < NT; ++d) {
-        const int ch = ((2 * d + ((lr & 3) >> 1)) ^ swz<D>(vrow)) * 16 + (lr & 1) * 8;     // (+ 4 rows: the same swizzle)
-        const char* a = vtile + vrow * (2 * D) + ch;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)a);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a + 4 * (2 * D)));
-        u32x4_a vw;
-        const u32x2_a l2 = __builtin_bit_cast(u32x2_a, lo), h2 = __builtin_bit_cast(u32x2_a, hi);
-        vw[0] = l2[0]; vw[1] = l2[1]; vw[2] = h2[0]; vw[3] = h2[1];
-        if (masked) {
-            // a hidden key's weight is 0, but 0 times NaN or infinity is not: such elements of V are taken out of the matrix product
-            // (and added below for the rows that do see them)
-            unsigned odd = 0;
+    for (int t = 0; t < RT; ++t) R.l[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), pb[t], R.l[t], 0, 0, 0);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) R.o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[d]), pb[t], R.o[t][d], 0, 0, 0);
+}
+
+// Does a fragment of V hold an infinity or a NaN?  (Both halves of every word: exponent bits all set = 0x7f80 or more without the sign.)
+template <int D>
+__device__ __forceinline__ bool any_odd(const u32x4_a (&vf)[D / 16]) {
+    typedef short s16x2_a __attribute__((ext_vector_type(2)));
+    s16x2_a top = {0, 0};
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = __builtin_elementwise_max(top, __builtin_bit_cast(s16x2_a, vf[d][w] & 0x7fff7fffu));
+    return __ballot(top[0] >= 0x7f80 || top[1] >= 0x7f80) != 0;
+}
+
+// Where some of the block's pairs are hidden and V holds infinities or NaN: a hidden key's weight is 0, but 0 times those is not.  They
+// are taken out of V's fragments, and what they make of the rows that do see them is added here: a product of their places with the
+// weights' signs (1 where a weight is not 0) counts, for every output, the infinities of either sign and the NaN among its keys.
+template <int D, int RT>
+__device__ __forceinline__ void take_out_odd(Rows<D, RT>& R, u32x4_a (&vf)[D / 16], const bf16x8 (&pb)[RT]) {
+    u32x4_a seen[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const unsigned p = __builtin_bit_cast(u32x4_a, pb[t])[w];
+            seen[t][w] = ((p & 0x7fffu) ? 0x3f80u : 0u) | ((p & 0x7fff0000u) ? 0x3f800000u : 0u);
+        }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+#pragma unroll
+        for (int kind = 0; kind < 3; ++kind) {          // +infinity, -infinity, NaN
+            u32x4_a at;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const bool b0 = (vw[w] & 0x7f80u) == 0x7f80u, b1 = (vw[w] & 0x7f800000u) == 0x7f800000u;
-                odd |= (b0 || b1) ? 1u : 0u;
-                vw[w] = (b0 ? 0u : vw[w] & 0xffffu) | (b1 ? 0u : vw[w] & 0xffff0000u);
+                const unsigned lo = vf[d][w] & 0xffffu, hi = vf[d][w] >> 16;
+                const bool l = kind == 0 ? lo == 0x7f80u : kind == 1 ? lo == 0xff80u : (lo & 0x7fffu) > 0x7f80u;
+                const bool h = kind == 0 ? hi == 0x7f80u : kind == 1 ? hi == 0xff80u : (hi & 0x7fffu) > 0x7f80u;
+                at[w] = (l ? 0x3f80u : 0u) | (h ? 0x3f800000u : 0u);
             }
-            if (__ballot(odd)) {
-                for (int key = 0; key < 32; ++key) {
+            const float add = kind == 0 ? -NEG_INF : kind == 1 ? NEG_INF : __builtin_nanf("");
 #pragma unroll
-                    for (int t = 0; t < RT; ++t) {
-                        const u32x4_a pw = __builtin_bit_cast(u32x4_a, pb[t]);
-                        const int src = (key >> 3) * 16 + lr;                                // the lane that holds this row's weight
-                        const unsigned word = (key & 6) == 0 ? pw[0] : (key & 6) == 2 ? pw[1] : (key & 6) == 4 ? pw[2] : pw[3];
-                        const unsigned w = __shfl((int)word, src, 64);
-                        const bool seen = ((key & 1 ? w >> 16 : w) & 0x7fffu) != 0;
+            for (int t = 0; t < RT; ++t) {
+                const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, at), __builtin_bit_cast(bf16x8, seen[t]),
+                                                                        f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int col = 16 * d + lq * 4 + r;
-                            const unsigned short bits = *reinterpret_cast<const unsigned short*>(
-                                vtile + key * (2 * D) + (((col >> 3) ^ swz<D>(key)) << 4) + (col & 7) * 2);
-                            if (seen && (bits & 0x7f80) == 0x7f80) R.o[t][d][r] += bf16_bits_to_f32(bits);
-                        }
-                    }
-                }
+                for (int r = 0; r < 4; ++r) R.o[t][d][r] += n[r] > 0.0f ? add : 0.0f;
             }
         }
-        const bf16x8 vf = __builtin_bit_cast(bf16x8, vw);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) R.o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[t], R.o[t][d], 0, 0, 0);
+        for (int w = 0; w < 4; ++w) {
+            const unsigned v = vf[d][w];
+            vf[d][w] = ((v & 0x7f80u) == 0x7f80u ? 0u : v & 0xffffu) | ((v & 0x7f800000u) == 0x7f800000u ? 0u : v & 0xffff0000u);
+        }
     }
 }
 
@@ -325,24 +409,26 @@ struct TileWalk {
 
 // normalise and store the wave's rows, or leave its state for the join
 template <int D, int RT>
-__device__ __forceinline__ void store_rows(const TextArgs& p, Rows<D, RT>& R, int64_t part_row0, int split, int64_t rows_all, int row0, int lane) {
+__device__ __forceinline__ void store_rows(const TextArgs& p, Rows<D, RT>& R, int b, int head0, int64_t part_row0, int split, int64_t rows_all, int row0,
+                                           int lane) {
     const int lr = lane & 15, lq = lane >> 4;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-        float l = R.l[t] + __shfl_xor(R.l[t], 16, 64);
-        l += __shfl_xor(l, 32, 64);
-        if (R.out_off[t] < 0) continue;
+        const float l = R.l[t][0];
+        const int in = row0 + t * 16 + lr, qi = in / p.pack, hg = in - qi * p.pack;
+        if (qi >= p.Sq) continue;
         if (p.splits == 1) {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            unsigned short* dst = p.out + b * p.ob + (int64_t)qi * p.os + (int64_t)(head0 + hg) * D + lq * 4;
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) {
                 bf16x4 v;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] = (bf16_t)(l == 0.0f ? 0.0f : R.o[t][d][r] * inv);
-                *reinterpret_cast<bf16x4*>(p.out + R.out_off[t] + d * 16 + lq * 4) = v;
+                *reinterpret_cast<bf16x4*>(dst + d * 16) = v;
             }
         } else {
-            const int64_t row = (int64_t)split * rows_all + part_row0 + row0 + t * 16 + lr;
+            const int64_t row = (int64_t)split * rows_all + part_row0 + in;
 #pragma unroll
             for (int d = 0; d < D / 16; ++d) *reinterpret_cast<f32x4*>(p.part + row * D + d * 16 + lq * 4) = R.o[t][d];
             if (lq == 0) {
@@ -361,7 +447,7 @@ __host__ __device__ __forceinline__ int bias_window(int pack) { return TKEYS + (
 
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
     constexpr int OPER = TKEYS * 2 * D;                 // one operand tile, bytes
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -401,83 +487,120 @@ __global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
 
     const unsigned short* Kh = p.k + b * p.kb + (int64_t)hk * p.kh;
     const unsigned short* Vh = p.v + b * p.vb + (int64_t)hk * p.vh;
-    constexpr int PER = 64 / (D / 8), PIECES = TKEYS / PER / 4;       // rows per 1 KiB piece, pieces per wave and operand
-    auto issue = [&](int t, int stage) {
-        char* ks = smem + stage * 2 * OPER + wave * PIECES * 1024;
+    // a tile's requests in two parts (K, V), so that neither stands in front of the arithmetic as one burst.  A piece is 1 KiB = PER
+    // rows; of the swizzle's row bits two lie inside a piece and bit 3 is the same for a piece: i / 2 (D = 128: 4 rows), i (D = 64: 8).
+    constexpr int PER = 64 / (D / 8), PIECES = TKEYS / PER / 4;
+    const int vr = wave * PIECES * PER + lane / (D / 8), vc = (lane % (D / 8)) ^ swz<D>(lane / (D / 8));
+    const int ks2 = (int)p.ks * 2, vs2 = (int)p.vs * 2;
+    const int koff = vr * ks2 + vc * 16, voff = vr * vs2 + vc * 16;
+    const int flip = ((vc ^ swz<D>(8)) - vc) * 16;                 // chunk offset of a piece whose rows have bit 3 set, minus the other's
+    const unsigned lds_wave = lds_address(smem) + wave * PIECES * 1024;
+    const int klane = k_lane<D>(lane), vlane = v_lane<D>(lane);
+    auto issue = [&](int t, int stage, int part) {
+        const unsigned to = lds_wave + (stage * 2 + part) * OPER;
+        const int step2 = part ? vs2 : ks2, left = p.Sk - t * TKEYS;
+        const u32x4_s rs = rows_resource<D>((part ? Vh : Kh) + (int64_t)t * (TKEYS / 2) * step2, part ? (int)p.vs : (int)p.ks, left < TKEYS ? left : TKEYS);
+        int off = part ? voff : koff;
+        asm volatile("" : "+v"(off));             // (the pieces' offsets are made here, not kept in registers over the loop)
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int r = (wave * PIECES + i) * PER + lane / (D / 8), cs = lane % (D / 8);
-            int key = t * TKEYS + r;
-            key = key < p.Sk ? key : p.Sk - 1;
-            glds16t(Kh + (int64_t)key * p.ks + ((cs ^ swz<D>(r)) << 3), ks + i * 1024);
-            glds16t(Vh + (int64_t)key * p.vs + ((cs ^ swz<D>(r)) << 3), ks + OPER + i * 1024);
-        }
+        for (int i = 0; i < PIECES; ++i) dma16(rs, off + ((i * PER) & 8 ? flip : 0) + i * PER * step2, to + i * 1024);
     };
     // bias window of tile t: entry w of head g = bias at distance 64 t - position(q_last) + w, in the log2 domain.  Finite values stay
-    // finite there (the lowest float times log2 e would not): rows that are biased down as a whole keep their order.
-    float* wins = reinterpret_cast<float*>(smem + 4 * OPER);
+    // finite there (the lowest float times log2 e would not): rows that are biased down as a whole keep their order.  Fetched in front of
+    // a tile's requests, written behind the previous tile's arithmetic.
+    float* wins = reinterpret_cast<float*>(smem + 4 * OPER + 512);
     const int64_t p_last = first_position(p, b) + q_last;
-    auto stage_bias = [&](int t, int stage) {
-        float* dst = wins + stage * p.pack * win;
-        for (int i = tid; i < p.pack * win; i += 256) {
-            const int g = i / win, w = i - g * win;
-            int64_t dist = (int64_t)t * TKEYS - p_last + w;
-            dist = dist < -p.reach ? -p.reach : dist > p.reach ? p.reach : dist;
-            const float v = p.bias[(int64_t)(head0 + g) * (2 * p.reach + 1) + p.reach + (int)dist];
-            const float big = 3.4028234663852886e38f;
-            dst[i] = fabsf(v) <= big ? fminf(fmaxf(v * LOG2E, -big), big) : v;
+    constexpr int NB = BIAS ? 3 : 1;                  // entries per thread: pack * win <= 8 * 81
+    int bsrc[NB], bw[NB];
+    float bv[NB];
+    if (BIAS) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int at = tid + 256 * i < p.pack * win ? tid + 256 * i : p.pack * win - 1;
+            const int g = at / win;
+            bw[i] = at - g * win;
+            bsrc[i] = (head0 + g) * (2 * p.reach + 1) + p.reach;
         }
+    }
+    auto fetch_bias = [&](int t) {
+        const int64_t far = (int64_t)t * TKEYS - p_last;
+        const int from = far < -0x40000000 ? -0x40000000 : far > 0x40000000 ? 0x40000000 : (int)far;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+            if (256 * i < p.pack * win) {
+                int dist = from + bw[i];
+                dist = dist < -p.reach ? -p.reach : dist > p.reach ? p.reach : dist;
+                bv[i] = p.bias[bsrc[i] + dist];
+            }
+    };
+    auto write_bias = [&](int stage) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+            if (tid + 256 * i < p.pack * win) wins[stage * p.pack * win + tid + 256 * i] = log2_bias(bv[i]);
+    };
+    int* const tile_docs = reinterpret_cast<int*>(smem + 4 * OPER);      // [2][64]: the documents of a tile's keys
+    auto issue_docs = [&](int t, int stage) {
+        const int left = p.Sk - t * TKEYS;
+        words_to_lds(p.kv_docs + b * p.kd_ld + t * TKEYS, left < TKEYS ? left : TKEYS, lane * 4, tile_docs + stage * 64);
     };
 
     int dlo, dhi, nlo = 0, nhi = 0;
     int t = walk.next(lane, dlo, dhi);
     int stage = 0;
     if (t >= 0) {
-        issue(t, 0);
-        if (BIAS) stage_bias(t, 0);
+        if (BIAS) fetch_bias(t);
+        issue(t, 0, 0);
+        issue(t, 0, 1);
+        if (p.q_docs && wave == 0) issue_docs(t, 0);
+        if (BIAS) write_bias(0);
     }
+    // One loop over 32-key blocks, two to a tile (nested loops made the compiler keep a second copy of the accumulators).
+    int tn = -1, blk = 0;
+    bool mine = false, masked = false;
     while (t >= 0) {
-        const int tn = walk.next(lane, nlo, nhi);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (tn >= 0) {
-            issue(tn, stage ^ 1);
-            if (BIAS) stage_bias(tn, stage ^ 1);
-        }
-        const char* kt0 = smem + stage * 2 * OPER;
-        const int key0 = t * TKEYS;
-        const bool mine = key0 < R.lim_hi && (!p.q_docs || (dlo <= R.doc_hi && dhi >= R.doc_lo));
-        if (mine) {
-            const bool masked = !(key0 + TKEYS <= R.lim_lo && (!p.q_docs || (dlo == dhi && R.doc_lo == R.doc_hi && dlo == R.doc_lo)));
-#pragma unroll
-            for (int blk = 0; blk < 2; ++blk) {
-                bf16x8 kf[2][D / 32];
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-                    const int row = blk * 32 + 8 * (lr >> 2) + 4 * kt + (lr & 3);
-#pragma unroll
-                    for (int s = 0; s < D / 32; ++s)
-                        kf[kt][s] = *reinterpret_cast<const bf16x8*>(kt0 + row * (2 * D) + (((s * 4 + lq) ^ swz<D>(row)) << 4));
-                }
-                int docs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (masked && p.q_docs) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int key = key0 + blk * 32 + 8 * lq + e;
-                        docs[e] = p.kv_docs[b * p.kd_ld + (key < p.Sk ? key : p.Sk - 1)];
-                    }
-                }
-                block_step<D, 2, CAP, BIAS>(p, R, kf, kt0 + OPER + blk * 32 * (2 * D), key0 + blk * 32, masked, docs,
-                                            wins + stage * p.pack * win + blk * 32 + 8 * lq, lane);
+        if (blk == 0) {
+            tn = walk.next(lane, nlo, nhi);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (tn >= 0) {
+                if (BIAS) fetch_bias(tn);
+                issue(tn, stage ^ 1, 0);
+                if (p.q_docs && wave == 0) issue_docs(tn, stage ^ 1);
             }
+            const int first = t * TKEYS;
+            mine = __builtin_amdgcn_readfirstlane((int)(first < R.lim_hi && (!p.q_docs || (dlo <= R.doc_hi && dhi >= R.doc_lo)))) != 0;
+            masked = __builtin_amdgcn_readfirstlane((int)!(first + TKEYS <= R.lim_lo && (!p.q_docs || (dlo == dhi && R.doc_lo == R.doc_hi && dlo == R.doc_lo)))) != 0;
         }
-        t = tn;
-        dlo = nlo;
-        dhi = nhi;
-        stage ^= 1;
+        if (mine) {
+            const int at = stage * 2 * OPER + blk * 32 * (2 * D), key0 = t * TKEYS + blk * 32;
+            bf16x8 kf[2][D / 32], pb[2];
+            u32x4_a vf[D / 16];
+            float s[2][8];
+            read_k<D>(smem, at + klane, kf);
+            block_qk<D, 2>(R, kf, s);
+            read_v<D>(smem, at + OPER + vlane, vf);       // in flight under the softmax
+            int docs[8];
+            if (masked && p.q_docs) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) docs[e] = tile_docs[stage * 64 + blk * 32 + 8 * lq + e];
+            }
+            block_softmax<D, 2, CAP, BIAS>(p, R, s, pb, key0, masked, docs, wins + stage * p.pack * win + blk * 32 + 8 * lq, lane);
+            if (masked && any_odd<D>(vf)) take_out_odd<D, 2>(R, vf, pb);
+            block_pv<D, 2>(R, vf, pb);
+        }
+        if (blk == 0) {
+            if (tn >= 0) issue(tn, stage ^ 1, 1);
+        } else {
+            if (BIAS && tn >= 0) write_bias(stage ^ 1);
+            t = tn;
+            dlo = nlo;
+            dhi = nhi;
+            stage ^= 1;
+        }
+        blk ^= 1;
     }
-    store_rows<D, 2>(p, R, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, tile * TROWS + wave * 32, lane);
+    store_rows<D, 2>(p, R, b, head0, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, tile * TROWS + wave * 32, lane);
 }
 
 // ---- up to 16 rows: the keys are what is long -----------------------------------------------------------------------------------
@@ -485,7 +608,7 @@ __global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
 // (a row's 2 D bytes are read whole), its V block through a private double buffer in LDS.  No barrier until the four states are joined.
 template <int D, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
     constexpr int OPER = 32 * 2 * D;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -509,6 +632,8 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
     float* const win_mine = reinterpret_cast<float*>(smem + 8 * OPER) + wave * p.pack * win;
     const int64_t p_last = first_position(p, b) + p.Sq - 1;
     constexpr int PER = 64 / (D / 8), PIECES = 32 / PER;
+    const int vr = lane / (D / 8), vc = (lane % (D / 8)) ^ swz<D>(vr), voff = vr * (int)p.vs * 2 + vc * 16;
+    const int flip = ((vc ^ swz<D>(8)) - vc) * 16;
     auto load_k = [&](int blk, bf16x8 (&kf)[2][D / 32]) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
@@ -518,14 +643,13 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
             for (int s = 0; s < D / 32; ++s) kf[kt][s] = *reinterpret_cast<const bf16x8*>(Kh + (int64_t)key * p.ks + (s * 4 + lq) * 8);
         }
     };
+    const unsigned lds_mine = lds_address(mine);
+    const int vlane = v_lane<D>(lane);
     auto load_v = [&](int blk, int stage) {
+        const int left = p.Sk - blk * 32;
+        const u32x4_s rs = rows_resource<D>(Vh + (int64_t)blk * 32 * p.vs, (int)p.vs, left < 32 ? left : 32);
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const int r = i * PER + lane / (D / 8), cs = lane % (D / 8);
-            int key = blk * 32 + r;
-            key = key < p.Sk ? key : p.Sk - 1;
-            glds16t(Vh + (int64_t)key * p.vs + ((cs ^ swz<D>(r)) << 3), mine + stage * OPER + i * 1024);
-        }
+        for (int i = 0; i < PIECES; ++i) dma16(rs, voff + ((i * PER) & 8 ? flip : 0) + i * PER * (int)p.vs * 2, lds_mine + stage * OPER + i * 1024);
     };
     bf16x8 kf[2][D / 32];
     int blk = b0 + wave, stage = 0;
@@ -552,14 +676,12 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
                 if (w < 32 + span) {
                     int64_t dist = (int64_t)key0 - p_last + w;
                     dist = dist < -p.reach ? -p.reach : dist > p.reach ? p.reach : dist;
-                    const float v = p.bias[(int64_t)(head0 + g) * (2 * p.reach + 1) + p.reach + (int)dist];
-                    const float big = 3.4028234663852886e38f;
-                    win_mine[i] = fabsf(v) <= big ? fminf(fmaxf(v * LOG2E, -big), big) : v;
+                    win_mine[i] = log2_bias(p.bias[(int64_t)(head0 + g) * (2 * p.reach + 1) + p.reach + (int)dist]);
                 }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        int docs[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        int docs[8];
         const bool masked = key0 + 32 > R.lim_lo || p.q_docs;
         if (p.q_docs) {
 #pragma unroll
@@ -568,7 +690,14 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
                 docs[e] = p.kv_docs[b * p.kd_ld + (key < p.Sk ? key : p.Sk - 1)];
             }
         }
-        block_step<D, 1, CAP, BIAS>(p, R, now, mine + stage * OPER, key0, masked, docs, win_mine + 8 * lq, lane);
+        float s[1][8];
+        bf16x8 pb[1];
+        u32x4_a vf[D / 16];
+        read_v<D>(smem, wave * 2 * OPER + stage * OPER + vlane, vf);
+        block_qk<D, 1>(R, now, s);
+        block_softmax<D, 1, CAP, BIAS>(p, R, s, pb, key0, masked, docs, win_mine + 8 * lq, lane);
+        if (masked && any_odd<D>(vf)) take_out_odd<D, 1>(R, vf, pb);
+        block_pv<D, 1>(R, vf, pb);
     }
     // ---- join the four waves' states through LDS: wave 0 takes the others in their order
     __syncthreads();
@@ -579,7 +708,7 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
 #pragma unroll
         for (int d = 0; d < NT; ++d) ox[((wave - 1) * NT + d) * 64 + lane] = R.o[0][d];
         mx[(wave - 1) * 128 + lane] = R.m[0];
-        mx[(wave - 1) * 128 + 64 + lane] = R.l[0];
+        mx[(wave - 1) * 128 + 64 + lane] = R.l[0][0];
     }
     __syncthreads();
     if (wave > 0) return;
@@ -589,11 +718,11 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
         const float n = fmaxf(R.m[0], m2), ref = n == NEG_INF ? 0.0f : n;
         const float a1 = __builtin_amdgcn_exp2f(R.m[0] - ref), a2 = __builtin_amdgcn_exp2f(m2 - ref);
         R.m[0] = n;
-        R.l[0] = R.l[0] * a1 + l2 * a2;
+        R.l[0][0] = R.l[0][0] * a1 + l2 * a2;
 #pragma unroll
         for (int d = 0; d < NT; ++d) R.o[0][d] = R.o[0][d] * a1 + ox[(w * NT + d) * 64 + lane] * a2;
     }
-    store_rows<D, 1>(p, R, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, 0, lane);
+    store_rows<D, 1>(p, R, b, head0, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, 0, lane);
 }
 
 // one wave per row: the splits' states in their order
@@ -685,7 +814,7 @@ int launch_text(const TextArgs& p, const Plan& n, hipStream_t st) {
         ea_count("attention_text_few");
         hipLaunchKernelGGL((attention_text_few_kernel<D, CAP, BIAS>), dim3((unsigned)sets, (unsigned)n.splits), dim3(256), lds, st, p);
     } else {
-        const int lds = 4 * oper + 2 * win;
+        const int lds = 4 * oper + 512 + 2 * win;
         if (hipFuncSetAttribute((const void*)attention_text_kernel<D, CAP, BIAS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
             return ea_check_launch("ea_attention_text_bf16");
         ea_count(n.splits > 1 ? "attention_text_split" : "attention_text");
@@ -728,7 +857,7 @@ extern "C" int ea_attention_text_bf16(const ea_bf16* q, const ea_bf16* k, const 
                "ea_attention_text_bf16: bad sizes (batch %d, heads %d / %d, queries %d, keys %d)", batch, q_heads, kv_heads, q_len, kv_len);
     EA_REQUIRE(scale > 0.0f && scale <= 3.4e38f, "ea_attention_text_bf16: scale must be positive and finite");
     EA_REQUIRE(cap >= 0.0f && cap <= 3.4e38f, "ea_attention_text_bf16: cap must be positive and finite, or 0 for none");
-    EA_REQUIRE(!bias || (reach >= 0 && reach <= 0x3fffffff), "ea_attention_text_bf16: bad reach %d", reach);
+    EA_REQUIRE(!bias || (reach >= 0 && reach <= 0x3fffffff && (2 * (int64_t)reach + 1) * q_heads <= 0x7fffffff), "ea_attention_text_bf16: bad reach %d", reach);
     EA_REQUIRE((q_docs == nullptr) == (kv_docs == nullptr), "ea_attention_text_bf16: q_docs and kv_docs come together");
     EA_REQUIRE(!prefix || causal, "ea_attention_text_bf16: a prefix needs causal order");
     if (q_len == 0) return EA_OK;
@@ -737,6 +866,7 @@ extern "C" int ea_attention_text_bf16(const ea_bf16* q, const ea_bf16* k, const 
     EA_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0, "ea_attention_text_bf16: 16-byte alignment");
     for (int i = 0; i < 11; ++i)
         EA_REQUIRE(strides[i] % 8 == 0 && strides[i] >= 0, "ea_attention_text_bf16: strides must be non-negative multiples of 8 elements");
+    EA_REQUIRE(strides[5] < (1 << 24) && strides[8] < (1 << 24), "ea_attention_text_bf16: row strides of k and v must be below 2^24 elements");
     const Plan n = plan_of(batch, q_heads, kv_heads, q_len, kv_len, head_dim, q_docs != nullptr);
     EA_REQUIRE(n.part_bytes + n.range_bytes == 0 ||
                    (workspace && workspace_bytes >= n.part_bytes + n.range_bytes && (uintptr_t)workspace % 16 == 0),

@@ -707,10 +707,10 @@ def attention_causal_gqa(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, seq
 
 def _strided(t: torch.Tensor):
     """(t, its batch / head / row strides) as ea_attention_text_bf16 reads them: unit inner stride, strides multiples of 8 (those of
-    one-element axes do not count), 16-byte aligned -- or a contiguous copy where t is not like that."""
+    one-element axes do not count), rows less than 2^24 apart, 16-byte aligned -- or a contiguous copy where t is not like that."""
     sh, (b, h, s, d) = t.shape, t.stride()
     b, h, s = b if sh[0] > 1 else 0, h if sh[1] > 1 else 0, s if sh[2] > 1 else 0
-    if d != 1 or (b | h | s) & 7 or t.data_ptr() & 15:
+    if d != 1 or (b | h | s) & 7 or s >= 1 << 24 or t.data_ptr() & 15:
         t = t.contiguous()
         if t.data_ptr() & 15:
             t = t.clone()

@@ -415,7 +415,7 @@ int ea_attention_causal_gqa_bf16(const ea_bf16* q, const ea_bf16* k, const ea_bf
  * result whatever they are (a key hidden from one query may hold a NaN that another query sees).
  *   q bf16 [batch, q_heads, q_len, D], k / v bf16 [batch, kv_heads, kv_len, D]: any batch, head and row strides; out bf16
  *   [batch, q_len, q_heads * D] by batch and row stride.  strides: HOST array of 11 element strides -- q batch, head, row; k ..;
- *   v ..; out batch, row -- non-negative multiples of 8; pointers 16-byte aligned.  D = 64 or 128; head h reads kv head
+ *   v ..; out batch, row -- non-negative multiples of 8, k and v row strides below 2^24; pointers 16-byte aligned.  D = 64 or 128; head h reads kv head
  *   h / (q_heads / kv_heads).  bias fp32 [q_heads][2 reach + 1] or NULL (lowest-float entries keep their order, -inf hides);
  *   q_docs / kv_docs int32 with row strides q_docs_ld / kv_docs_ld; prefix, valid, q_start int32 [batch] or NULL (prefix: causal only).
  * scale > 0.  workspace: ea_attention_text_workspace_bytes() bytes of the caller's (documents = 1 when q_docs is given), 0 for many
