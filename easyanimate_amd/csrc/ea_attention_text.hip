@@ -114,13 +114,23 @@ __device__ __forceinline__ int wave_max(int v) {
     for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
     return v;
 }
-__device__ __forceinline__ int64_t first_position(const TextArgs& p, int b) { return p.q_start ? p.q_start[b] : (int64_t)p.Sk - p.Sq; }
-__device__ __forceinline__ int key_limit(const TextArgs& p, int b, int qi) {
-    int64_t lim = p.Sk;
-    if (p.valid) lim = p.valid[b] < lim ? p.valid[b] : lim;
+// what a batch element's masks are: position of its first query, keys that exist, keys every query sees
+struct Seq {
+    int64_t first;
+    int keys, prefix;
+};
+__device__ __forceinline__ Seq seq_of(const TextArgs& p, int b) {
+    Seq s;
+    s.first = p.q_start ? p.q_start[b] : (int64_t)p.Sk - p.Sq;
+    s.keys = p.valid && p.valid[b] < p.Sk ? p.valid[b] : p.Sk;
+    s.prefix = p.prefix ? p.prefix[b] : 0;
+    return s;
+}
+__device__ __forceinline__ int key_limit(const TextArgs& p, const Seq& s, int qi) {
+    int64_t lim = s.keys;
     if (p.causal) {
-        int64_t c = first_position(p, b) + qi + 1;
-        if (p.prefix && p.prefix[b] > c) c = p.prefix[b];
+        int64_t c = s.first + qi + 1;
+        c = s.prefix > c ? s.prefix : c;
         lim = c < lim ? c : lim;
     }
     return lim > 0 ? (int)lim : 0;
@@ -128,7 +138,7 @@ __device__ __forceinline__ int key_limit(const TextArgs& p, int b, int qi) {
 
 // head0: first query head of the packed set; row0: first row of this wave; qlast: last query of the workgroup's tile
 template <int D, int RT>
-__device__ __forceinline__ void load_rows(const TextArgs& p, Rows<D, RT>& R, int b, int head0, int row0, int qlast, int win, int lane) {
+__device__ __forceinline__ void load_rows(const TextArgs& p, Rows<D, RT>& R, const Seq& seq, int b, int head0, int row0, int qlast, int win, int lane) {
     const int lr = lane & 15, lq = lane >> 4;
     R.lim_lo = 0x7fffffff;
     R.lim_hi = 0;
@@ -144,7 +154,7 @@ __device__ __forceinline__ void load_rows(const TextArgs& p, Rows<D, RT>& R, int
         const unsigned short* src = p.q + b * p.qb + (int64_t)(head0 + hg) * p.qh + (int64_t)qi * p.qs + lq * 8;
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) R.q[t][s] = *reinterpret_cast<const bf16x8*>(src + s * 32);
-        R.lim[t] = key_limit(p, b, qi);
+        R.lim[t] = key_limit(p, seq, qi);
         R.doc[t] = p.q_docs ? p.q_docs[b * p.qd_ld + qi] : 0;
         R.back[t] = hg * win + (qlast - qi);
         R.lim_lo = min(R.lim_lo, R.lim[t]);
@@ -463,11 +473,10 @@ __global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
     const int q_last = min((tile * TROWS + TROWS - 1) / p.pack, p.Sq - 1);
     const int win = BIAS ? bias_window(p.pack) : 1;
 
-    Rows<D, 2> R;
-    load_rows<D, 2>(p, R, b, head0, tile * TROWS + wave * 32, q_last, win, lane);
+    const Seq seq = seq_of(p, b);
 
     // ---- the workgroup's keys: up to the greatest limit (the limit grows with the query), documents of its queries
-    const int lim_all = key_limit(p, b, q_last);
+    const int lim_all = key_limit(p, seq, q_last);
     const int nt = (lim_all + TKEYS - 1) / TKEYS;
     TileWalk walk;
     walk.range = nullptr;
@@ -509,7 +518,7 @@ __global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
     // finite there (the lowest float times log2 e would not): rows that are biased down as a whole keep their order.  Fetched in front of
     // a tile's requests, written behind the previous tile's arithmetic.
     float* wins = reinterpret_cast<float*>(smem + 4 * OPER + 512);
-    const int64_t p_last = first_position(p, b) + q_last;
+    const int64_t p_last = seq.first + q_last;
     constexpr int NB = BIAS ? 3 : 1;                  // entries per thread: pack * win <= 8 * 81
     int bsrc[NB], bw[NB];
     float bv[NB];
@@ -554,6 +563,8 @@ __global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
         if (p.q_docs && wave == 0) issue_docs(t, 0);
         if (BIAS) write_bias(0);
     }
+    Rows<D, 2> R;                                     // (behind the first tile's requests: both are under way together)
+    load_rows<D, 2>(p, R, seq, b, head0, tile * TROWS + wave * 32, q_last, win, lane);
     // One loop over 32-key blocks, two to a tile (nested loops made the compiler keep a second copy of the accumulators).
     int tn = -1, blk = 0;
     bool mine = false, masked = false;
@@ -619,18 +630,16 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
     const int head0 = set * p.pack, hk = head0 / p.group;
     const int split = blockIdx.y;
     const int rows = p.Sq * p.pack;
-    const int win = BIAS ? bias_window(p.pack) : 1;
-
-    Rows<D, 1> R;
-    load_rows<D, 1>(p, R, b, head0, 0, p.Sq - 1, win, lane);
-    const int nb = (key_limit(p, b, p.Sq - 1) + 31) / 32;
+    const int win = 31 + p.Sq;                           // bias window of a block: its 32 keys against every query
+    const Seq seq = seq_of(p, b);
+    const int nb = (key_limit(p, seq, p.Sq - 1) + 31) / 32;
     const int b0 = (int)((int64_t)nb * split / p.splits), b1 = (int)((int64_t)nb * (split + 1) / p.splits);
 
     const unsigned short* Kh = p.k + b * p.kb + (int64_t)hk * p.kh;
     const unsigned short* Vh = p.v + b * p.vb + (int64_t)hk * p.vh;
     char* const mine = smem + wave * 2 * OPER;
     float* const win_mine = reinterpret_cast<float*>(smem + 8 * OPER) + wave * p.pack * win;
-    const int64_t p_last = first_position(p, b) + p.Sq - 1;
+    const int64_t p_last = seq.first + p.Sq - 1;
     constexpr int PER = 64 / (D / 8), PIECES = 32 / PER;
     const int vr = lane / (D / 8), vc = (lane % (D / 8)) ^ swz<D>(vr), voff = vr * (int)p.vs * 2 + vc * 16;
     const int flip = ((vc ^ swz<D>(8)) - vc) * 16;
@@ -651,51 +660,71 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) dma16(rs, voff + ((i * PER) & 8 ? flip : 0) + i * PER * (int)p.vs * 2, lds_mine + stage * OPER + i * 1024);
     };
+    constexpr int NB = BIAS ? 5 : 1;                     // window entries per lane: pack * win <= 8 * 31 + 16
+    int bsrc[NB], bw[NB];
+    float bv[NB];
+    if (BIAS) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int at = lane + 64 * i < p.pack * win ? lane + 64 * i : p.pack * win - 1, g = at / win;
+            bw[i] = at - g * win;
+            bsrc[i] = (head0 + g) * (2 * p.reach + 1) + p.reach;
+        }
+    }
+    int docs[8];
+    // a block's requests: what is small and looked at first (bias window, documents) in front
+    auto request = [&](int blk, bf16x8 (&kf)[2][D / 32], int stage) {
+        if (BIAS) {
+            const int64_t far = (int64_t)blk * 32 - p_last;
+            const int from = far < -0x40000000 ? -0x40000000 : far > 0x40000000 ? 0x40000000 : (int)far;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                if (64 * i < p.pack * win) {
+                    int dist = from + bw[i];
+                    dist = dist < -p.reach ? -p.reach : dist > p.reach ? p.reach : dist;
+                    bv[i] = p.bias[bsrc[i] + dist];
+                }
+        }
+        if (p.q_docs) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int key = blk * 32 + 8 * lq + e;
+                docs[e] = p.kv_docs[b * p.kd_ld + (key < p.Sk ? key : p.Sk - 1)];
+            }
+        }
+        load_k(blk, kf);
+        load_v(blk, stage);
+    };
     bf16x8 kf[2][D / 32];
     int blk = b0 + wave, stage = 0;
-    if (blk < b1) {
-        load_k(blk, kf);
-        load_v(blk, 0);
-    }
+    if (blk < b1) request(blk, kf, 0);
+    Rows<D, 1> R;                                        // (behind the first block's requests)
+    load_rows<D, 1>(p, R, seq, b, head0, 0, p.Sq - 1, win, lane);
     for (; blk < b1; blk += 4, stage ^= 1) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         bf16x8 now[2][D / 32];
+        int now_docs[8];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int s = 0; s < D / 32; ++s) now[kt][s] = kf[kt][s];
-        if (blk + 4 < b1) {
-            load_k(blk + 4, kf);
-            load_v(blk + 4, stage ^ 1);
-        }
-        const int key0 = blk * 32;
-        if (BIAS) {
-            const int span = p.Sq - 1;           // this block's window: 32 keys against every query
-            for (int i = lane; i < p.pack * win; i += 64) {
-                const int g = i / win, w = i - g * win;
-                if (w < 32 + span) {
-                    int64_t dist = (int64_t)key0 - p_last + w;
-                    dist = dist < -p.reach ? -p.reach : dist > p.reach ? p.reach : dist;
-                    win_mine[i] = log2_bias(p.bias[(int64_t)(head0 + g) * (2 * p.reach + 1) + p.reach + (int)dist]);
-                }
-            }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        }
-        int docs[8];
-        const bool masked = key0 + 32 > R.lim_lo || p.q_docs;
-        if (p.q_docs) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int key = key0 + 8 * lq + e;
-                docs[e] = p.kv_docs[b * p.kd_ld + (key < p.Sk ? key : p.Sk - 1)];
-            }
+        for (int e = 0; e < 8; ++e) now_docs[e] = docs[e];
+        if (BIAS) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                if (lane + 64 * i < p.pack * win) win_mine[lane + 64 * i] = log2_bias(bv[i]);
         }
+        if (blk + 4 < b1) request(blk + 4, kf, stage ^ 1);
+        const int key0 = blk * 32;
+        const bool masked = key0 + 32 > R.lim_lo || p.q_docs;
+        if (BIAS) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         float s[1][8];
         bf16x8 pb[1];
         u32x4_a vf[D / 16];
         read_v<D>(smem, wave * 2 * OPER + stage * OPER + vlane, vf);
         block_qk<D, 1>(R, now, s);
-        block_softmax<D, 1, CAP, BIAS>(p, R, s, pb, key0, masked, docs, win_mine + 8 * lq, lane);
+        block_softmax<D, 1, CAP, BIAS>(p, R, s, pb, key0, masked, now_docs, win_mine + 8 * lq, lane);
         if (masked && any_odd<D>(vf)) take_out_odd<D, 1>(R, vf, pb);
         block_pv<D, 1>(R, vf, pb);
     }
@@ -725,27 +754,38 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
     store_rows<D, 1>(p, R, b, head0, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, 0, lane);
 }
 
-// one wave per row: the splits' states in their order
+// One workgroup per row: the splits' weights first (one thread each), then 256 / D threads per output element over the splits, each
+// taking every (256 / D)-th, and their sums in a fixed order.
+constexpr int MAX_SPLITS = 256;
 template <int D>
 __global__ __launch_bounds__(256) void attention_text_join_kernel(TextArgs p) {
-    const int lane = threadIdx.x & 63;
-    const int64_t rows_all = (int64_t)p.B * p.Hq * p.Sq;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows_all) return;
+    constexpr int PARTS = 256 / D;
+    __shared__ float wm[MAX_SPLITS], wl[MAX_SPLITS], o_part[PARTS][D];
+    const int tid = threadIdx.x;
+    const int64_t rows_all = (int64_t)p.B * p.Hq * p.Sq, row = blockIdx.x;
     const float* ml = p.part + (int64_t)p.splits * rows_all * D;
-    float top = NEG_INF;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[(s * rows_all + row) * 2]);
-    const float ref = top == NEG_INF ? 0.0f : top;
-    float l = 0.f, o[D / 64];
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-        const int64_t r = s * rows_all + row;
-        const float a = __builtin_amdgcn_exp2f(ml[r * 2] - ref);
-        l += ml[r * 2 + 1] * a;
-#pragma unroll
-        for (int e = 0; e < D / 64; ++e) o[e] += p.part[r * D + e * 64 + lane] * a;
+    if (tid < p.splits) {
+        wm[tid] = ml[((int64_t)tid * rows_all + row) * 2];
+        wl[tid] = ml[((int64_t)tid * rows_all + row) * 2 + 1];
     }
+    __syncthreads();
+    float top = NEG_INF;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, wm[s]);
+    const float ref = top == NEG_INF ? 0.0f : top;
+    __syncthreads();
+    if (tid < p.splits) wm[tid] = __builtin_amdgcn_exp2f(wm[tid] - ref);
+    __syncthreads();
+    const int d = tid % D, part = tid / D;
+    const float* src = p.part + row * D + d;
+    float o = 0.f, l = 0.f;
+#pragma unroll 8
+    for (int s = part; s < p.splits; s += PARTS) o += src[(int64_t)s * rows_all * D] * wm[s];
+    o_part[part][d] = o;
+    for (int s = 0; s < p.splits; ++s) l += wl[s] * wm[s];
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) o += o_part[i][d];
     // row = ((b * sets + set) * Sq + query) * pack + head of the set
     const int64_t rows = (int64_t)p.Sq * p.pack;
     const int nsets = p.Hq / p.pack;
@@ -753,9 +793,7 @@ __global__ __launch_bounds__(256) void attention_text_join_kernel(TextArgs p) {
     const int in = (int)(row - set_all * rows), qi = in / p.pack, hg = in % p.pack;
     const int64_t b = set_all / nsets;
     const int head = (int)(set_all % nsets) * p.pack + hg;
-    unsigned short* dst = p.out + b * p.ob + (int64_t)qi * p.os + (int64_t)head * D;
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) dst[e * 64 + lane] = f32_to_bf16_bits(l == 0.0f ? 0.0f : o[e] / l);
+    p.out[b * p.ob + (int64_t)qi * p.os + (int64_t)head * D + d] = f32_to_bf16_bits(l == 0.0f ? 0.0f : o / l);
 }
 
 // least and greatest document of every 64-key tile: one wave each
@@ -792,7 +830,7 @@ Plan plan_of(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs) {
     int64_t s = (512 + wgs - 1) / wgs;
     const int64_t most = ((int64_t)Sk + 255) / 256;
     s = s < most ? s : most;
-    s = s < 1 ? 1 : s > 256 ? 256 : s;
+    s = s < 1 ? 1 : s > MAX_SPLITS ? MAX_SPLITS : s;
     if (!n.few && wgs >= 192) s = 1;
     n.splits = (int)s;
     n.part_bytes = n.splits > 1 ? n.splits * sets * rows * (D + 2) * 4 : 0;
@@ -803,7 +841,7 @@ Plan plan_of(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs) {
 template <int D, bool CAP, bool BIAS>
 int launch_text(const TextArgs& p, const Plan& n, hipStream_t st) {
     const int oper = (n.few ? 32 : TKEYS) * 2 * D;
-    const int win = BIAS ? bias_window(p.pack) * p.pack * 4 : 0;
+    const int win = !BIAS ? 0 : n.few ? (31 + p.Sq) * p.pack * 4 : bias_window(p.pack) * p.pack * 4;
     const int64_t sets = (int64_t)p.B * (p.Hq / p.pack);
     if (n.few) {
         const int tail = 3 * 16 * D * 4 + 3 * 2 * 64 * 4;                 // the join's image
@@ -822,7 +860,7 @@ int launch_text(const TextArgs& p, const Plan& n, hipStream_t st) {
     }
     if (n.splits > 1) {
         const int64_t rows_all = (int64_t)p.B * p.Hq * p.Sq;
-        hipLaunchKernelGGL(attention_text_join_kernel<D>, dim3((unsigned)((rows_all + 3) / 4)), dim3(256), 0, st, p);
+        hipLaunchKernelGGL(attention_text_join_kernel<D>, dim3((unsigned)rows_all), dim3(256), 0, st, p);
     }
     return ea_check_launch("ea_attention_text_bf16");
 }
@@ -836,7 +874,7 @@ int dispatch_text(const TextArgs& p, const Plan& n, hipStream_t st) {
 bool sizes_ok(int B, int Hq, int Hkv, int Sq, int Sk, int D) {
     if (!(B > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Sq >= 0 && Sk >= 0 && (D == 64 || D == 128))) return false;
     // rows of a packed set stay in 32 bits, grids within a launch's limits
-    return (int64_t)Sq * BIAS_PACK_MAX <= 0x7fffff00 && Sk <= 0x7fffff00 && B <= 65535 && (int64_t)B * Hq * (((int64_t)Sq + 7) / 8) <= 0x7fffffff;
+    return (int64_t)Sq * BIAS_PACK_MAX <= 0x7fffff00 && Sk <= 0x7fffff00 && B <= 65535 && (int64_t)B * Hq * Sq <= 0x7fffffff;
 }
 
 }  // namespace
