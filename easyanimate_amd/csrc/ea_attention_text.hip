@@ -451,12 +451,18 @@ __device__ __forceinline__ void store_rows(const TextArgs& p, Rows<D, RT>& R, in
 }
 
 // ---- 128 rows per workgroup ------------------------------------------------------------------------------------------------------
+// Bound by issue slots, not by memory or the matrix pipe: for one wave and 32-key block at D = 128 the matrix instructions take 544
+// clocks of about 1240, the softmax 98 vector and 74 scalar instructions; two waves of a SIMD cover each other in part (matrix pipe
+// busy 44 %).  1024 TFLOP/s at 28 / 4 heads, 8192 tokens, D = 128; 820 at 32 / 32 heads, 4096 tokens (333 us; cap 375 us, bias 353 us);
+// 755 at D = 64 (2 x 32 heads, 4096 tokens: 364 us).  At D = 64 the registers of three workgroups per CU are given room for: 490
+// against 554 us with a cap, 452 against 533 us with a bias, the plain forms alike.  Measured and not taken: a tile's two blocks
+// overlapped inside a wave (spills at D = 128, 407 against 364 us at D = 64), K fragments read a block ahead (slower on all sizes).
 constexpr int TROWS = 128, TKEYS = 64;
 // floats per head of a tile's bias window: its 64 keys against every query of the row tile
 __host__ __device__ __forceinline__ int bias_window(int pack) { return TKEYS + (TROWS - 1) / pack + 2; }
 
 template <int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void attention_text_kernel(TextArgs p) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(TextArgs p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     constexpr int OPER = TKEYS * 2 * D;                 // one operand tile, bytes
     const int tid = threadIdx.x, lane = tid & 63;
@@ -874,7 +880,7 @@ int dispatch_text(const TextArgs& p, const Plan& n, hipStream_t st) {
 bool sizes_ok(int B, int Hq, int Hkv, int Sq, int Sk, int D) {
     if (!(B > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Sq >= 0 && Sk >= 0 && (D == 64 || D == 128))) return false;
     // rows of a packed set stay in 32 bits, grids within a launch's limits
-    return (int64_t)Sq * BIAS_PACK_MAX <= 0x7fffff00 && Sk <= 0x7fffff00 && B <= 65535 && (int64_t)B * Hq * Sq <= 0x7fffffff;
+    return (int64_t)Sq * BIAS_PACK_MAX <= 0x7fffff00 && Sk <= 0x7fffff00 && B <= 65535 && (int64_t)B * Hq * Sq <= 0x7fffffff && (int64_t)B * Hq < (1 << 24);
 }
 
 }  // namespace
@@ -893,8 +899,9 @@ extern "C" int ea_attention_text_bf16(const ea_bf16* q, const ea_bf16* k, const 
     EA_REQUIRE(head_dim == 64 || head_dim == 128, "ea_attention_text_bf16: head_dim %d (64 and 128 are built)", head_dim);
     EA_REQUIRE(sizes_ok(batch, q_heads, kv_heads, q_len, kv_len, head_dim),
                "ea_attention_text_bf16: bad sizes (batch %d, heads %d / %d, queries %d, keys %d)", batch, q_heads, kv_heads, q_len, kv_len);
-    EA_REQUIRE(scale > 0.0f && scale <= 3.4e38f, "ea_attention_text_bf16: scale must be positive and finite");
-    EA_REQUIRE(cap >= 0.0f && cap <= 3.4e38f, "ea_attention_text_bf16: cap must be positive and finite, or 0 for none");
+    EA_REQUIRE(scale > 0.0f && scale <= 1e30f, "ea_attention_text_bf16: scale must be positive and at most 1e30");
+    EA_REQUIRE(cap == 0.0f || (cap >= 1e-30f && cap <= 1e30f && scale / cap <= 1e30f),
+               "ea_attention_text_bf16: cap must be 0 for none, or between 1e-30 and 1e30 and at least 1e-30 of the scale");
     EA_REQUIRE(!bias || (reach >= 0 && reach <= 0x3fffffff && (2 * (int64_t)reach + 1) * q_heads <= 0x7fffffff), "ea_attention_text_bf16: bad reach %d", reach);
     EA_REQUIRE((q_docs == nullptr) == (kv_docs == nullptr), "ea_attention_text_bf16: q_docs and kv_docs come together");
     EA_REQUIRE(!prefix || causal, "ea_attention_text_bf16: a prefix needs causal order");
@@ -904,6 +911,8 @@ extern "C" int ea_attention_text_bf16(const ea_bf16* q, const ea_bf16* k, const 
     EA_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0, "ea_attention_text_bf16: 16-byte alignment");
     for (int i = 0; i < 11; ++i)
         EA_REQUIRE(strides[i] % 8 == 0 && strides[i] >= 0, "ea_attention_text_bf16: strides must be non-negative multiples of 8 elements");
+    EA_REQUIRE((batch == 1 || strides[9] >= (int64_t)q_heads * head_dim) && (q_len == 1 || strides[10] >= (int64_t)q_heads * head_dim),
+               "ea_attention_text_bf16: rows of out overlap (strides %lld, %lld)", (long long)strides[9], (long long)strides[10]);
     EA_REQUIRE(strides[5] < (1 << 24) && strides[8] < (1 << 24), "ea_attention_text_bf16: row strides of k and v must be below 2^24 elements");
     const Plan n = plan_of(batch, q_heads, kv_heads, q_len, kv_len, head_dim, q_docs != nullptr);
     EA_REQUIRE(n.part_bytes + n.range_bytes == 0 ||

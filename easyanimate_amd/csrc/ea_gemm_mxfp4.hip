@@ -526,6 +526,8 @@ extern "C" int ea_gemm_mxfp4(const uint8_t* A, const uint8_t* A_scales, const ea
                              int64_t gate_batch_stride, int epilogue, void* workspace, int64_t workspace_bytes, void* stream) {
     EA_REQUIRE(batch > 0 && batch <= 65535 && M >= 0 && N > 0 && K > 0, "ea_gemm_mxfp4: bad sizes (batch %d, M %d, N %d, K %d)", batch, M, N, K);
     EA_REQUIRE(N % 8 == 0 && ldc % 8 == 0 && c_batch_stride % 8 == 0, "ea_gemm_mxfp4: N (%d), ldc and c_batch_stride must be multiples of 8", N);
+    EA_REQUIRE((M <= 1 || ldc >= N) && (batch == 1 || c_batch_stride >= N), "ea_gemm_mxfp4: rows of C overlap (ldc %lld, batch stride %lld)",
+               (long long)ldc, (long long)c_batch_stride);
     EA_REQUIRE(M <= 0x7fffff00 && N <= 0x7fffff00 && (((int64_t)M + 63) / 64) * (((int64_t)N + 63) / 64) <= 0x7fffffff &&
                    (int64_t)batch * M * (N / 4) <= (int64_t)0x7fffffff * 256,
                "ea_gemm_mxfp4: product too large for one launch (M %d, N %d)", M, N);

@@ -730,7 +730,8 @@ def attention_text(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
       q_docs / kv_docs   int32 [B, Sq] / [B, Sk]: only keys of the query's document (ids arbitrary; packed documents are skipped fast)
       valid        int32 [B]: keys that exist
       q_start      int32 [B]: position of the first query (default Sk - Sq: the queries are the last tokens)
-    A query that sees no key gives zeros.  One new token against a long cache is split over the GPU.  (ea_attention_text_bf16)"""
+    A query that sees no key gives zeros.  One new token against a long cache is split over the GPU.  out must not overlap q, k or v.
+    (ea_attention_text_bf16)"""
     _chk(q, _BF16, "q"); _chk(k, _BF16, "k"); _chk(v, _BF16, "v")
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"q, k, v: expected [B, H, S, D] with k and v alike, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -740,8 +741,8 @@ def attention_text(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not belong together (batch, head_dim, heads a multiple of kv heads)")
     if D not in (64, 128):
         raise ValueError(f"head_dim {D}: 64 and 128 are built")
-    if not (0.0 < scale < float("inf")) or not (0.0 <= cap < float("inf")):
-        raise ValueError(f"scale must be positive and finite, cap positive and finite or 0 (got {scale}, {cap})")
+    if not (0.0 < scale <= 1e30) or not (cap == 0.0 or (1e-30 <= cap <= 1e30 and scale <= 1e30 * cap)):
+        raise ValueError(f"scale must be positive and at most 1e30, cap 0 or between 1e-30 and 1e30 (got {scale}, {cap})")
     reach = 0
     if bias is not None:
         _chk(bias, _F32, "bias")
@@ -764,6 +765,8 @@ def attention_text(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
         _chk(out, _BF16, "out")
         if out.shape != (B, Sq, Hq * D) or out.stride(2) != 1:
             raise ValueError(f"out: expected [{B}, {Sq}, {Hq * D}] with unit inner stride, got {tuple(out.shape)}, strides {out.stride()}")
+        if (B > 1 and out.stride(0) < Hq * D) or (Sq > 1 and out.stride(1) < Hq * D):
+            raise ValueError(f"out: rows overlap (strides {out.stride()})")
         if B == 0 or Sq == 0:
             return out
         if Sk == 0:

@@ -415,10 +415,10 @@ int ea_attention_causal_gqa_bf16(const ea_bf16* q, const ea_bf16* k, const ea_bf
  * result whatever they are (a key hidden from one query may hold a NaN that another query sees).
  *   q bf16 [batch, q_heads, q_len, D], k / v bf16 [batch, kv_heads, kv_len, D]: any batch, head and row strides; out bf16
  *   [batch, q_len, q_heads * D] by batch and row stride.  strides: HOST array of 11 element strides -- q batch, head, row; k ..;
- *   v ..; out batch, row -- non-negative multiples of 8, k and v row strides below 2^24; pointers 16-byte aligned.  D = 64 or 128; head h reads kv head
- *   h / (q_heads / kv_heads).  bias fp32 [q_heads][2 reach + 1] or NULL (lowest-float entries keep their order, -inf hides);
+ *   v ..; out batch, row -- non-negative multiples of 8, k and v row strides below 2^24, those of out at least q_heads * D; out must not overlap
+ *   the inputs; pointers 16-byte aligned.  D = 64 or 128; head h reads kv head h / (q_heads / kv_heads).  bias fp32 [q_heads][2 reach + 1] or NULL (lowest-float entries keep their order, -inf hides);
  *   q_docs / kv_docs int32 with row strides q_docs_ld / kv_docs_ld; prefix, valid, q_start int32 [batch] or NULL (prefix: causal only).
- * scale > 0.  workspace: ea_attention_text_workspace_bytes() bytes of the caller's (documents = 1 when q_docs is given), 0 for many
+ * 0 < scale <= 1e30; cap 0 (none) or 1e-30 .. 1e30, at least 1e-30 of the scale.  workspace: ea_attention_text_workspace_bytes() bytes of the caller's (documents = 1 when q_docs is given), 0 for many
  * shapes; calls that may run at the same time need one each.  Results do not depend on timing. */
 int64_t ea_attention_text_workspace_bytes(int batch, int q_heads, int kv_heads, int q_len, int kv_len, int head_dim, int documents);
 int ea_attention_text_bf16(const ea_bf16* q, const ea_bf16* k, const ea_bf16* v, ea_bf16* out, const int64_t* strides, int batch,

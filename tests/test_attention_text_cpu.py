@@ -22,10 +22,10 @@ def test_refuses(lib_built):
               (q, _t(2, 2, 9, 128), _t(2, 2, 9, 128)), (_t(2, 4, 5, 80), _t(2, 2, 9, 80), _t(2, 2, 9, 80))):
         with pytest.raises(ValueError):
             ops.attention_text(*a, 0.125)
-    for s in (0.0, -1.0, float("inf"), float("nan")):
+    for s in (0.0, -1.0, 2e30, float("inf"), float("nan")):
         with pytest.raises(ValueError):
             ops.attention_text(q, k, k, s)
-    for kw in (dict(cap=-1.0), dict(cap=float("nan")), dict(cap=float("inf")), dict(bias=_t(4, 8, dtype=torch.float32)), dict(bias=_t(3, 9, dtype=torch.float32)),
+    for kw in (dict(cap=-1.0), dict(cap=1e-31), dict(cap=1e31), dict(cap=float("nan")), dict(cap=float("inf")), dict(bias=_t(4, 8, dtype=torch.float32)), dict(bias=_t(3, 9, dtype=torch.float32)),
                dict(bias=_t(4, 18, dtype=torch.float32)[:, ::2]), dict(q_docs=i(2, 5)), dict(kv_docs=i(2, 9)), dict(q_docs=i(2, 9), kv_docs=i(2, 9)),
                dict(q_docs=i(2, 5), kv_docs=i(9, 2).t()), dict(prefix=i(2)), dict(prefix=i(3), causal=True), dict(valid=i(1)), dict(q_start=i(2, 1))):
         with pytest.raises(ValueError):
@@ -46,10 +46,12 @@ def test_abi_refuses(lib_built):
         return lib.ea_attention_text_bf16(q, k, v, out, ctypes.addressof(arr) if arr else None, B, Hq, Hkv, Sq, Sk, D, scale, causal, cap, bias, reach, qd, kd, 0,
                                           0, prefix, valid, start, ws, wsb, None)
 
-    st = lambda i, v: tuple(v if n == i else 64 for n in range(11))
+    st = lambda i, v: tuple(v if n == i else 256 for n in range(11))
     bad = [dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(strides=None), dict(q=p + 8), dict(out=p + 2), dict(B=0), dict(Hkv=3), dict(Hkv=0),
            dict(Sq=-1), dict(Sk=0), dict(Sk=-5), dict(D=80), dict(D=256), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
-           dict(cap=-1.0), dict(cap=float("nan")), dict(bias=p, reach=-1), dict(qd=p), dict(kd=p), dict(prefix=p), dict(strides=st(1, 4)), dict(strides=st(9, -8)),
+           dict(cap=-1.0), dict(cap=float("nan")), dict(bias=p, reach=-1), dict(qd=p), dict(kd=p), dict(prefix=p), dict(strides=st(1, 4)), dict(strides=st(9, -8)), dict(strides=st(5, 1 << 24)), dict(strides=st(8, 1 << 24)),
+           dict(strides=st(10, 248)), dict(strides=st(9, 0), B=2), dict(scale=2e30), dict(cap=1e-31), dict(cap=1e31), dict(cap=1e-20, scale=1e12), dict(B=65535, Hq=512),
+           
            dict(qd=p, kd=p, Sq=40), dict(Sq=64, Sk=4096), dict(Sq=64, Sk=4096, ws=p, wsb=16), dict(Sq=0x7fffffff), dict(B=70000)]
     for kw in bad:
         assert call(**kw) == -1, kw

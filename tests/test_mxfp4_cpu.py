@@ -66,7 +66,7 @@ def test_abi_refuses(lib_built):
         return lib.ea_gemm_mxfp4(A, As, X, W, Ws, bias, C, res, gate, batch, M, N, K, lda, abs_, ldc, cbs, ldres, rbs, gbs, epi, ws, wsb, None)
 
     bad = [dict(A=None), dict(As=None), dict(W=None), dict(Ws=None), dict(C=None), dict(X=p), dict(N=12), dict(N=0), dict(K=0), dict(M=-1),
-           dict(batch=0), dict(batch=70000), dict(ldc=12), dict(cbs=4), dict(epi=4), dict(epi=-1), dict(epi=2), dict(epi=2, res=p), dict(C=p + 8),
+           dict(batch=0), dict(batch=70000), dict(ldc=8), dict(X=p, A=None, As=None, batch=2, ws=p, wsb=1 << 20), dict(ldc=12), dict(cbs=4), dict(epi=4), dict(epi=-1), dict(epi=2), dict(epi=2, res=p), dict(C=p + 8),
            dict(A=p + 4), dict(As=p + 4), dict(bias=p + 4), dict(A=None, As=None, X=p, M=17), dict(A=None, As=None, X=p, K=60),
            dict(A=None, As=None, X=p, lda=60), dict(A=None, As=None, X=p, lda=-8), dict(A=None, As=None, X=p + 1), dict(M=100, K=16384),
            dict(M=100, K=16384, ws=p, wsb=64), dict(M=100, K=16384, ws=p + 8, wsb=1 << 30),
