@@ -114,6 +114,14 @@ def bf16_weight(p, k_pad: int | None = None):
     return derived(p, f"bf16w{k_pad}", make)
 
 
+def mxfp4_weight(p):
+    """The microscaled 4-bit storage (ops.Mxfp4, 17 / 32 byte per weight) of a Linear weight [N, K], cached like every derived weight:
+    laid out again after load_state_dict, in-place writes or a move; writes through `.data` need invalidate_weight_cache(), which the
+    pipelines call at the start of each run."""
+    from . import ops
+    return derived(p, "mxfp4", lambda t: ops.mxfp4_quantize(t.to(torch.bfloat16)))
+
+
 def kblocked_weight(p):
     """The K-blocked copy [K / 64, N, 64] of a bf16 Linear weight [N, K] (ops.gemm_kblocked; cached like every derived weight:
     load_state_dict / in-place writes are seen through the version counter).  `.data` writes are not, so outside a

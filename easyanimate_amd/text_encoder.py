@@ -15,7 +15,11 @@ Qwen2-VL / Qwen2 modelling code (pinned by tests/test_text_encoder_gpu.py agains
 `Qwen2VLTextEncoderHIP(hf_model)` wraps the loaded transformers model WITHOUT copying its weights and answers the one call the
 pipelines make: `enc(input_ids=, attention_mask=, output_hidden_states=True).hidden_states[-2]`, plus `.device` / `.dtype`.
 Linear layers run on ea_gemm_bf16 (residual adds in its epilogue), norms on ea_rmsnorm_bf16, the rest on ea_text.hip.
-Text-only: image / video inputs are refused (the EasyAnimate pipelines never pass any).  There is no CPU fallback."""
+Text-only: image / video inputs are refused (the EasyAnimate pipelines never pass any).  There is no CPU fallback.
+
+`weights="mxfp4"` runs the same layers with 4-bit Linear layers (ops.gemm_mxfp4: weights and activations in blocks of 32 e2m1 codes
+under one power-of-two scale; a layer's q / k / v and gate / up products share one quantised input) and ops.attention_text, which reads
+V as the projection left it: a fast approximation, 0.1 to 0.2 relative error per product.  The default is the bf16 path above."""
 from __future__ import annotations
 
 import types
@@ -25,7 +29,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from ._params import f32, gemm_weight
+from ._params import f32, gemm_weight, mxfp4_weight
 
 
 def _find_text_model(hf_model):
@@ -47,14 +51,18 @@ def _find_text_model(hf_model):
 
 
 class Qwen2VLTextEncoderHIP(nn.Module):
-    def __init__(self, hf_model, padded_positions: str = "arange"):
+    def __init__(self, hf_model, padded_positions: str = "arange", weights: str = "bf16"):
         """padded_positions: the rotary position of the right-PADDED slots (real tokens are 0 .. n-1 either way; the DiT consumes
         the padded rows too, transformer3d.py:1502).  "arange" = transformers 5.x (the installed version: text-only prompts get
-        the text model's own arange(S)); "cumsum_fill1" = transformers 4.46 - 4.5x (get_rope_index: cumsum(mask) - 1, padding -> 1)."""
+        the text model's own arange(S)); "cumsum_fill1" = transformers 4.46 - 4.5x (get_rope_index: cumsum(mask) - 1, padding -> 1).
+        weights: "bf16", or "mxfp4" for 4-bit Linear layers (laid out at the first call)."""
         super().__init__()
         if padded_positions not in ("arange", "cumsum_fill1"):
             raise ValueError(f"padded_positions must be 'arange' or 'cumsum_fill1', not {padded_positions!r}")
+        if weights not in ("bf16", "mxfp4"):
+            raise ValueError(f"weights must be 'bf16' or 'mxfp4', not {weights!r}")
         self.padded_positions = padded_positions
+        self.weights = weights
         self.hf = hf_model                                 # (registered: .to() / offload hooks reach the shared parameters)
         text = _find_text_model(hf_model)
         cfg = text.config
@@ -67,6 +75,8 @@ class Qwen2VLTextEncoderHIP(nn.Module):
         self.theta = float(rp.get("rope_theta", None) or getattr(cfg, "rope_theta", None) or 10000.0)
         if self.head_dim not in (64, 128):
             raise NotImplementedError(f"Qwen2VLTextEncoderHIP: head_dim {self.head_dim} (ea_attention_causal_gqa_bf16 is built for 64 and 128)")
+        if weights == "mxfp4" and (self.hidden % 8 or cfg.intermediate_size % 8):
+            raise NotImplementedError(f"Qwen2VLTextEncoderHIP: weights='mxfp4' needs widths that are multiples of 8 (got {self.hidden}, {cfg.intermediate_size})")
         if getattr(cfg, "use_sliding_window", False):
             raise NotImplementedError("Qwen2VLTextEncoderHIP: sliding-window layers are not implemented (Qwen2-VL-7B does not use them)")
         if getattr(cfg, "hidden_act", "silu") != "silu":
@@ -92,6 +102,21 @@ class Qwen2VLTextEncoderHIP(nn.Module):
         if key not in self._ones:
             self._ones[key] = torch.ones(n, dtype=torch.float32, device=device)
         return self._ones[key]
+
+    def _layer_mxfp4(self, layer, h, B, S, cos, sin, valid):
+        att, mlp, D, Hq, Hkv = layer.self_attn, layer.mlp, self.head_dim, self.q_heads, self.kv_heads
+        ones = self._gate_ones(self.hidden, h.device)
+        fb = lambda lin: f32(lin.bias) if lin.bias is not None else None
+        lin = lambda a, l: ops.gemm_mxfp4(a, mxfp4_weight(l.weight), fb(l))
+        add = lambda a, l, res: ops.gemm_mxfp4(a, mxfp4_weight(l.weight), fb(l), ops.EPI_BIAS_GATE_RES, res=res, gate=ones)
+        n1 = ops.mxfp4_quantize(ops.rmsnorm(h, f32(layer.input_layernorm.weight), self.eps))
+        qh = ops.rope_half_scatter(lin(n1, att.q_proj), Hq, D, B, S, cos, sin)
+        kh = ops.rope_half_scatter(lin(n1, att.k_proj), Hkv, D, B, S, cos, sin)
+        v = lin(n1, att.v_proj).view(B, S, Hkv, D).transpose(1, 2)
+        a = ops.attention_text(qh, kh, v, D ** -0.5, causal=True, valid=valid)
+        h = add(a.view(B * S, Hq * D), att.o_proj, h)
+        n2 = ops.mxfp4_quantize(ops.rmsnorm(h, f32(layer.post_attention_layernorm.weight), self.eps))
+        return add(ops.silu_mul(lin(n2, mlp.gate_proj), lin(n2, mlp.up_proj)), mlp.down_proj, h)
 
     @torch.no_grad()
     def forward(self, input_ids: Optional[torch.Tensor] = None, attention_mask: Optional[torch.Tensor] = None,
@@ -130,10 +155,15 @@ class Qwen2VLTextEncoderHIP(nn.Module):
         ang = torch.cat([ang, ang], dim=-1).reshape(B * S, D)
         cos, sin = ang.cos().contiguous(), ang.sin().contiguous()
         s_pad = ops.round_up(S, 32)
-        vt = torch.zeros(B, Hkv, D, s_pad, dtype=torch.bfloat16, device=dev)
+        four = self.weights == "mxfp4"
+        vt = None if four else torch.zeros(B, Hkv, D, s_pad, dtype=torch.bfloat16, device=dev)
         h = x.reshape(B * S, d).contiguous()
         hidden_states = [x]
         for layer in text.layers:
+            if four:
+                h = self._layer_mxfp4(layer, h, B, S, cos, sin, valid)
+                hidden_states.append(h.view(B, S, d))
+                continue
             att, mlp = layer.self_attn, layer.mlp
             n1 = ops.rmsnorm(h, f32(layer.input_layernorm.weight), self.eps)
             q = ops.gemm(n1, gemm_weight(att.q_proj.weight), f32(att.q_proj.bias) if att.q_proj.bias is not None else None)
@@ -157,10 +187,10 @@ class Qwen2VLTextEncoderHIP(nn.Module):
         return types.SimpleNamespace(last_hidden_state=last, hidden_states=tuple(hidden_states) if output_hidden_states else None)
 
 
-def use_hip_text_encoder(pipeline, index: int = 0):
+def use_hip_text_encoder(pipeline, index: int = 0, weights: str = "bf16"):
     """Swap the transformers model in a pipeline's text_encoder slot for its device-library forward (weights shared)."""
     name = "text_encoder" if index == 0 else "text_encoder_2"
     enc = getattr(pipeline, name)
     if enc is not None and not isinstance(enc, Qwen2VLTextEncoderHIP):
-        setattr(pipeline, name, Qwen2VLTextEncoderHIP(enc))
+        setattr(pipeline, name, Qwen2VLTextEncoderHIP(enc, weights=weights))
     return getattr(pipeline, name)
