@@ -17,10 +17,10 @@
 // accumulators are hardly ever rescaled); P is rounded to bf16 for its product (a relative half step of 2^-8 each); the row sums are
 // those of the rounded weights, by one more product with ones, in fp32.
 //
-//   attention_text_kernel       128 rows per workgroup (four waves, 32 rows each), K / V tiles of 64 keys double-buffered in LDS by
+//   attention_text_kernel       128 or 64 rows per workgroup (four waves, 32 or 16 rows each), K / V tiles of 64 keys double-buffered in LDS by
 //                               LDS-DMA; tiles that no row of the workgroup sees are skipped (64 at a time for documents)
 //   attention_text_few_kernel   up to 16 rows: each of the four waves walks its own 32-key blocks, K straight into registers
-//   Both can split the keys over workgroups; attention_text_join_kernel combines the partial results in a fixed order.
+//   The few rows and the 64-row tiles can split the keys over workgroups; the join kernels combine the partial results in a fixed order.
 #include "ea_common.h"
 
 namespace {
@@ -450,20 +450,21 @@ __device__ __forceinline__ void store_rows(const TextArgs& p, Rows<D, RT>& R, in
     }
 }
 
-// ---- 128 rows per workgroup ------------------------------------------------------------------------------------------------------
+// ---- 128 or 64 rows per workgroup --------------------------------------------------------------------------------------------------
 // Bound by issue slots, not by memory or the matrix pipe: for one wave and 32-key block at D = 128 the matrix instructions take 544
 // clocks of about 1240, the softmax 98 vector and 74 scalar instructions; two waves of a SIMD cover each other in part (matrix pipe
 // busy 44 %).  1024 TFLOP/s at 28 / 4 heads, 8192 tokens, D = 128; 820 at 32 / 32 heads, 4096 tokens (333 us; cap 375 us, bias 353 us);
 // 755 at D = 64 (2 x 32 heads, 4096 tokens: 364 us).  At D = 64 the registers of three workgroups per CU are given room for: 490
 // against 554 us with a cap, 452 against 533 us with a bias, the plain forms alike.  Measured and not taken: a tile's two blocks
 // overlapped inside a wave (spills at D = 128, 407 against 364 us at D = 64), K fragments read a block ahead (slower on all sizes).
-constexpr int TROWS = 128, TKEYS = 64;
+constexpr int TKEYS = 64;
 // floats per head of a tile's bias window: its 64 keys against every query of the row tile
-__host__ __device__ __forceinline__ int bias_window(int pack) { return TKEYS + (TROWS - 1) / pack + 2; }
+__host__ __device__ __forceinline__ int bias_window(int trows, int pack) { return TKEYS + (trows - 1) / pack + 2; }
 
-template <int D, bool CAP, bool BIAS>
+template <int D, int RT, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(TextArgs p) {
     extern __shared__ __attribute__((aligned(1024))) char smem[];
+    constexpr int TROWS = 64 * RT;
     constexpr int OPER = TKEYS * 2 * D;                 // one operand tile, bytes
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
     const int rows = p.Sq * p.pack;
     const int q_first = tile * TROWS / p.pack;
     const int q_last = min((tile * TROWS + TROWS - 1) / p.pack, p.Sq - 1);
-    const int win = BIAS ? bias_window(p.pack) : 1;
+    const int win = BIAS ? bias_window(TROWS, p.pack) : 1;
 
     const Seq seq = seq_of(p, b);
 
@@ -569,8 +570,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
         if (p.q_docs && wave == 0) issue_docs(t, 0);
         if (BIAS) write_bias(0);
     }
-    Rows<D, 2> R;                                     // (behind the first tile's requests: both are under way together)
-    load_rows<D, 2>(p, R, seq, b, head0, tile * TROWS + wave * 32, q_last, win, lane);
+    Rows<D, RT> R;                                     // (behind the first tile's requests: both are under way together)
+    load_rows<D, RT>(p, R, seq, b, head0, tile * TROWS + wave * 16 * RT, q_last, win, lane);
     // One loop over 32-key blocks, two to a tile (nested loops made the compiler keep a second copy of the accumulators).
     int tn = -1, blk = 0;
     bool mine = false, masked = false;
@@ -591,20 +592,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
         }
         if (mine) {
             const int at = stage * 2 * OPER + blk * 32 * (2 * D), key0 = t * TKEYS + blk * 32;
-            bf16x8 kf[2][D / 32], pb[2];
+            bf16x8 kf[2][D / 32], pb[RT];
             u32x4_a vf[D / 16];
-            float s[2][8];
+            float s[RT][8];
             read_k<D>(smem, at + klane, kf);
-            block_qk<D, 2>(R, kf, s);
+            block_qk<D, RT>(R, kf, s);
             read_v<D>(smem, at + OPER + vlane, vf);       // in flight under the softmax
             int docs[8];
             if (masked && p.q_docs) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) docs[e] = tile_docs[stage * 64 + blk * 32 + 8 * lq + e];
             }
-            block_softmax<D, 2, CAP, BIAS>(p, R, s, pb, key0, masked, docs, wins + stage * p.pack * win + blk * 32 + 8 * lq, lane);
-            if (masked && any_odd<D>(vf)) take_out_odd<D, 2>(R, vf, pb);
-            block_pv<D, 2>(R, vf, pb);
+            block_softmax<D, RT, CAP, BIAS>(p, R, s, pb, key0, masked, docs, wins + stage * p.pack * win + blk * 32 + 8 * lq, lane);
+            if (masked && any_odd<D>(vf)) take_out_odd<D, RT>(R, vf, pb);
+            block_pv<D, RT>(R, vf, pb);
         }
         if (blk == 0) {
             if (tn >= 0) issue(tn, stage ^ 1, 1);
@@ -617,7 +618,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
         }
         blk ^= 1;
     }
-    store_rows<D, 2>(p, R, b, head0, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, tile * TROWS + wave * 32, lane);
+    store_rows<D, RT>(p, R, b, head0, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, tile * TROWS + wave * 16 * RT, lane);
 }
 
 // ---- up to 16 rows: the keys are what is long -----------------------------------------------------------------------------------
@@ -763,6 +764,43 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
 // One workgroup per row: the splits' weights first (one thread each), then 256 / D threads per output element over the splits, each
 // taking every (256 / D)-th, and their sums in a fixed order.
 constexpr int MAX_SPLITS = 256;
+// Up to 12 splits D / 4 threads per row: 8400 rows, 3 splits, 24 us altogether, 31 with a workgroup per row (448 rows, 64 splits: 31
+// against 23).
+template <int D>
+__device__ __forceinline__ unsigned short* out_row_of(const TextArgs& p, const int64_t row) {
+    // row = ((b * sets + set) * Sq + query) * pack + head of the set
+    const int64_t rows = (int64_t)p.Sq * p.pack;
+    const int nsets = p.Hq / p.pack;
+    const int64_t set_all = row / rows;
+    const int in = (int)(row - set_all * rows), qi = in / p.pack, hg = in % p.pack;
+    const int64_t b = set_all / nsets;
+    return p.out + b * p.ob + (int64_t)qi * p.os + (int64_t)((int)(set_all % nsets) * p.pack + hg) * D;
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void attention_text_join_rows_kernel(TextArgs p) {
+    const int64_t rows_all = (int64_t)p.B * p.Hq * p.Sq, row = (int64_t)blockIdx.x * (1024 / D) + threadIdx.x / (D / 4);
+    if (row >= rows_all) return;
+    const int d = threadIdx.x % (D / 4) * 4;
+    const float* src = p.part + row * D + d;
+    const float* ml = p.part + (int64_t)p.splits * rows_all * D + row * 2;
+    float m = NEG_INF, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[(int64_t)s * rows_all * 2]);
+    const float ref = m == NEG_INF ? 0.0f : m;
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+        const float w = __builtin_amdgcn_exp2f(ml[(int64_t)s * rows_all * 2] - ref);
+        l += ml[(int64_t)s * rows_all * 2 + 1] * w;
+        o += *reinterpret_cast<const f32x4*>(src + (int64_t)s * rows_all * D) * w;
+    }
+    bf16x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (bf16_t)(l == 0.0f ? 0.0f : o[r] / l);
+    *reinterpret_cast<bf16x4*>(out_row_of<D>(p, row) + d) = v;
+}
+
 template <int D>
 __global__ __launch_bounds__(256) void attention_text_join_kernel(TextArgs p) {
     constexpr int PARTS = 256 / D;
@@ -792,14 +830,7 @@ __global__ __launch_bounds__(256) void attention_text_join_kernel(TextArgs p) {
     if (part) return;
 #pragma unroll
     for (int i = 1; i < PARTS; ++i) o += o_part[i][d];
-    // row = ((b * sets + set) * Sq + query) * pack + head of the set
-    const int64_t rows = (int64_t)p.Sq * p.pack;
-    const int nsets = p.Hq / p.pack;
-    const int64_t set_all = row / rows;
-    const int in = (int)(row - set_all * rows), qi = in / p.pack, hg = in % p.pack;
-    const int64_t b = set_all / nsets;
-    const int head = (int)(set_all % nsets) * p.pack + hg;
-    p.out[b * p.ob + (int64_t)qi * p.os + (int64_t)head * D + d] = f32_to_bf16_bits(l == 0.0f ? 0.0f : o / l);
+    out_row_of<D>(p, row)[d] = f32_to_bf16_bits(l == 0.0f ? 0.0f : o / l);
 }
 
 // least and greatest document of every 64-key tile: one wave each
@@ -817,7 +848,7 @@ __global__ __launch_bounds__(64) void doc_range_kernel(const int* __restrict__ d
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 struct Plan {
-    int group, pack, few, row_tiles, key_tiles, splits;
+    int group, pack, few, rt, row_tiles, key_tiles, splits;
     int64_t part_bytes, range_bytes;
 };
 
@@ -830,14 +861,19 @@ Plan plan_of(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs) {
     const int64_t sets = (int64_t)B * (Hq / n.pack);
     n.few = rows <= 16;
     n.key_tiles = (int)(((int64_t)Sk + TKEYS - 1) / TKEYS);
-    n.row_tiles = n.few ? 1 : (int)((rows + TROWS - 1) / TROWS);
-    // split the keys while the workgroups do not fill the chip twice (256 CUs) and a split keeps at least 256 keys
+    // 64 rows per workgroup where 128 would leave CUs without a second one (1024 causal tokens of 28 heads: 26 against 32 us; 2048 tokens,
+    // 448 workgroups of 128 rows: 79 us, 108 with 64)
+    n.rt = sets * ((rows + 127) / 128) <= 256 ? 1 : 2;
+    n.row_tiles = n.few ? 1 : (int)((rows + 64 * n.rt - 1) / (64 * n.rt));
+    // Split the keys while all workgroups still run at once (two to each of 256 CUs; 256 queries of 28 heads, 8192 keys: 64 us with 4
+    // splits = 448 workgroups, 84 with 5) and a split keeps what pays for the join: 512 keys (128 queries, 4096 keys: 30 us; 38 with 256
+    // keys, 33 with 1024), 256 where few rows are joined.  From 192 workgroups of whole tiles on the join costs more than is gained
+    // (512 x 512: 15 against 24 us).
     const int64_t wgs = sets * n.row_tiles;
-    int64_t s = (512 + wgs - 1) / wgs;
-    const int64_t most = ((int64_t)Sk + 255) / 256;
+    int64_t s = 512 / wgs;
+    const int64_t most = ((int64_t)Sk + 255) / (n.few ? 256 : 512);
     s = s < most ? s : most;
-    s = s < 1 ? 1 : s > MAX_SPLITS ? MAX_SPLITS : s;
-    if (!n.few && wgs >= 192) s = 1;
+    s = s < 1 || (!n.few && wgs >= 192) ? 1 : s > MAX_SPLITS ? MAX_SPLITS : s;
     n.splits = (int)s;
     n.part_bytes = n.splits > 1 ? n.splits * sets * rows * (D + 2) * 4 : 0;
     n.range_bytes = docs && !n.few ? (int64_t)B * n.key_tiles * 8 : 0;
@@ -847,7 +883,7 @@ Plan plan_of(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs) {
 template <int D, bool CAP, bool BIAS>
 int launch_text(const TextArgs& p, const Plan& n, hipStream_t st) {
     const int oper = (n.few ? 32 : TKEYS) * 2 * D;
-    const int win = !BIAS ? 0 : n.few ? (31 + p.Sq) * p.pack * 4 : bias_window(p.pack) * p.pack * 4;
+    const int win = !BIAS ? 0 : n.few ? (31 + p.Sq) * p.pack * 4 : bias_window(64 * n.rt, p.pack) * p.pack * 4;
     const int64_t sets = (int64_t)p.B * (p.Hq / p.pack);
     if (n.few) {
         const int tail = 3 * 16 * D * 4 + 3 * 2 * 64 * 4;                 // the join's image
@@ -859,14 +895,18 @@ int launch_text(const TextArgs& p, const Plan& n, hipStream_t st) {
         hipLaunchKernelGGL((attention_text_few_kernel<D, CAP, BIAS>), dim3((unsigned)sets, (unsigned)n.splits), dim3(256), lds, st, p);
     } else {
         const int lds = 4 * oper + 512 + 2 * win;
-        if (hipFuncSetAttribute((const void*)attention_text_kernel<D, CAP, BIAS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+        const auto kernel = n.rt == 1 ? attention_text_kernel<D, 1, CAP, BIAS> : attention_text_kernel<D, 2, CAP, BIAS>;
+        if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
             return ea_check_launch("ea_attention_text_bf16");
-        ea_count(n.splits > 1 ? "attention_text_split" : "attention_text");
-        hipLaunchKernelGGL((attention_text_kernel<D, CAP, BIAS>), dim3((unsigned)(sets * n.row_tiles), (unsigned)n.splits), dim3(256), lds, st, p);
+        ea_count(n.rt == 2 ? "attention_text" : n.splits > 1 ? "attention_text_64_split" : "attention_text_64");      // (128 rows: never split)
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(sets * n.row_tiles), (unsigned)n.splits), dim3(256), lds, st, p);
     }
     if (n.splits > 1) {
         const int64_t rows_all = (int64_t)p.B * p.Hq * p.Sq;
-        hipLaunchKernelGGL(attention_text_join_kernel<D>, dim3((unsigned)rows_all), dim3(256), 0, st, p);
+        if (n.splits <= 12)
+            hipLaunchKernelGGL(attention_text_join_rows_kernel<D>, dim3((unsigned)((rows_all + 1024 / D - 1) / (1024 / D))), dim3(256), 0, st, p);
+        else
+            hipLaunchKernelGGL(attention_text_join_kernel<D>, dim3((unsigned)rows_all), dim3(256), 0, st, p);
     }
     return ea_check_launch("ea_attention_text_bf16");
 }

@@ -78,11 +78,28 @@ def check(q, k, v, scale, kern=None, **kw):
     kw.pop("out", None)
     want, err = plain(q, k, v, scale, **kw)
     got = got.cpu().double()
+    _inside(got, want, err)
+    # the same batch again and again, until there are enough workgroups for the 128-row tiles
+    B, Hq, Sq, _ = q.shape
+    pack = max(n for n in range(1, 9) if Hq // k.shape[1] % n == 0)
+    if Sq * pack > 16:
+        reps = 256 // (B * Hq // pack * ((Sq * pack + 127) // 128)) + 1
+        rep = lambda t: t.repeat(reps, *[1] * (t.dim() - 1))
+        _lib.reset_counters()
+        many = ops.attention_text(up(rep(q)), up(rep(k)), up(rep(v)), scale,
+                                  **{n: up(rep(t)) if n in ("q_docs", "kv_docs", "prefix", "valid", "q_start") and t is not None else up(t) for n, t in kw.items()})
+        assert _lib.counters().get("attention_text") == 1, _lib.counters()
+        many = many.view(reps, B, Sq, -1).cpu().double()
+        _inside(many[-1], want, err)
+        assert torch.equal(many[0].nan_to_num(), many[-1].nan_to_num())
+    return got
+
+
+def _inside(got, want, err):
     assert got.shape == want.shape
     assert torch.equal(torch.isnan(got), torch.isnan(want)), "NaN in other places"
     bad = ((got - want).abs() > err) & torch.isfinite(want)
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} outside, worst ratio {torch.nan_to_num((got - want).abs() / err).max().item():.3g}"
-    return got
 
 
 def make(B, Hq, Hkv, Sq, Sk, D, seed, spread=1.0):
@@ -145,7 +162,7 @@ def test_forms(name, D, Hq, Hkv, Sq, Sk):
     check(q, k, v, D ** -0.5, **form(name, 3, Hq, Sq, Sk, g))
 
 
-@pytest.mark.parametrize("Sq,Sk,kern", [(1, 5000, "attention_text_few"), (40, 3000, "attention_text_split"), (600, 600, None)])
+@pytest.mark.parametrize("Sq,Sk,kern", [(1, 5000, "attention_text_few"), (40, 3000, "attention_text_64_split"), (40, 9000, "attention_text_64_split"), (600, 600, "attention_text_64")])
 @pytest.mark.parametrize("name", ["cap", "all", "far_bias"])
 def test_long(Sq, Sk, kern, name):
     q, k, v, g = make(1, 4, 2, Sq, Sk, 128, Sq + Sk)
