@@ -175,8 +175,9 @@ __device__ __forceinline__ void load_rows(const TextArgs& p, Rows<D, RT>& R, con
 }
 
 // cap tanh(t / cap) log2(e) of t = s scale.  tanh(x) = 1 - 2 / (1 + e^2x): absolute error about cap 2^-22, so for a cap that is large
-// beside the scores (cap_wide: cap > 256) small x go through the odd series x - x^3/3 + 2x^5/15 - 17x^7/315 (|x| < 0.25: the next
+// beside the scores (cap > CAP_WIDE) small x go through the odd series x - x^3/3 + 2x^5/15 - 17x^7/315 (|x| < 0.25: the next
 // term is 6e-8 of x) instead.
+constexpr float CAP_WIDE = 256.0f;
 __device__ __forceinline__ float capped_log2(float s, float two_over, float c1, float half_over, bool wide) {
     const float e = __builtin_amdgcn_exp2f(s * two_over);
     float t = __builtin_fmaf(-2.0f * c1, __builtin_amdgcn_rcpf(e + 1.0f), c1);
@@ -233,35 +234,72 @@ __device__ __forceinline__ void block_qk(const Rows<D, RT>& R, const bf16x8 (&kf
         }
 }
 
-// Scores -> weights of one 32-key block, state updated.  win0: this lane's bias window position of key 8 lq of the block.
+// What a score still has to be multiplied with to be in the log2 domain, behind cap_and_bias.
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ float unit_of(const TextArgs& p) { return CAP || BIAS ? 1.0f : p.scale * LOG2E; }
+
+// Cap and bias of one 32-key block, to the log2 domain.  win0: this lane's bias window position of key 8 lq of the block.
+template <int D, int RT, bool CAP, bool BIAS, bool WIDE>
+__device__ __forceinline__ void cap_and_bias(const TextArgs& p, const Rows<D, RT>& R, float (&s)[RT][8], const float* win0) {
+    const float c = p.scale * LOG2E;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (CAP) s[t][e] = capped_log2(s[t][e], 2.0f * c / p.cap, p.cap * LOG2E, p.scale / p.cap, WIDE);
+            if (BIAS) s[t][e] = __builtin_fmaf(s[t][e], CAP ? 1.0f : c, win0[R.back[t] + e]);
+        }
+}
+// this lane's greatest score per row, and whether one has outgrown the reference maximum
+template <int D, int RT>
+__device__ __forceinline__ bool block_top(const Rows<D, RT>& R, const float (&s)[RT][8], const float unit, float (&top)[RT]) {
+    bool grow = false;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        top[t] = max2(max2(max2(s[t][0], s[t][1]), max2(s[t][2], s[t][3])), max2(max2(s[t][4], s[t][5]), max2(s[t][6], s[t][7]))) * unit;
+        grow = grow | (top[t] > R.m[t] + 8.0f);
+    }
+    return grow;
+}
+template <int D, int RT>
+__device__ __forceinline__ void block_grow(Rows<D, RT>& R, const float (&top)[RT]) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        float n = fmaxf(top[t], __shfl_xor(top[t], 16, 64));
+        n = fmaxf(n, __shfl_xor(n, 32, 64));
+        n = fmaxf(n, R.m[t]);
+        const float alpha = n == NEG_INF ? 1.0f : __builtin_amdgcn_exp2f(R.m[t] - n);
+        R.m[t] = n;
+        R.l[t] *= alpha;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) R.o[t][d] *= alpha;
+    }
+}
+template <int D, int RT>
+__device__ __forceinline__ void block_weights(const Rows<D, RT>& R, const float (&s)[RT][8], const float unit, bf16x8 (&pb)[RT]) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const float ref = R.m[t] == NEG_INF ? 0.0f : R.m[t];
+        u32x4_a pk;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], unit, -ref));
+            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e + 1], unit, -ref));
+            const f32x2 two = {p0, p1};
+            pk[e >> 1] = __builtin_bit_cast(unsigned, __builtin_convertvector(two, bf16x2));
+        }
+        pb[t] = __builtin_bit_cast(bf16x8, pk);
+    }
+}
+
+// Scores -> weights of one 32-key block, state updated.
 // masked: some pair of the block may be hidden; docs: this lane's 8 keys' documents (masked blocks of packed documents).
 template <int D, int RT, bool CAP, bool BIAS>
 __device__ __forceinline__ void block_softmax(const TextArgs& p, Rows<D, RT>& R, float (&s)[RT][8], bf16x8 (&pb)[RT], int key0, bool masked,
                                               const int (&docs)[8], const float* win0, int lane) {
     const int lq = lane >> 4;
-    const float c = p.scale * LOG2E;
-    // to the log2 domain where a cap or a bias makes the score more than a multiple of q.k
-    const float unit = CAP || BIAS ? 1.0f : c;                    // what a score still has to be multiplied with
-    if (CAP) {
-        const float c1 = p.cap * LOG2E, two_over = 2.0f * c / p.cap, half_over = p.scale / p.cap;
-        if (p.cap > 256.0f) {
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[t][e] = capped_log2(s[t][e], two_over, c1, half_over, true);
-        } else {
-#pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[t][e] = capped_log2(s[t][e], two_over, c1, half_over, false);
-        }
-    }
-    if (BIAS) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[t][e] = __builtin_fmaf(s[t][e], CAP ? 1.0f : c, win0[R.back[t] + e]);
-    }
+    if (CAP && p.cap > CAP_WIDE) cap_and_bias<D, RT, CAP, BIAS, true>(p, R, s, win0);
+    else cap_and_bias<D, RT, CAP, BIAS, false>(p, R, s, win0);
     if (masked) {
         if (p.q_docs) {
 #pragma unroll
@@ -276,40 +314,10 @@ __device__ __forceinline__ void block_softmax(const TextArgs& p, Rows<D, RT>& R,
             for (int e = 0; e < 8; ++e) s[t][e] = e < room ? s[t][e] : NEG_INF;
         }
     }
-    // move the reference maximum only when a row has outgrown it
     float top[RT];
-    bool grow = false;
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        top[t] = max2(max2(max2(s[t][0], s[t][1]), max2(s[t][2], s[t][3])), max2(max2(s[t][4], s[t][5]), max2(s[t][6], s[t][7]))) * unit;
-        grow = grow | (top[t] > R.m[t] + 8.0f);
-    }
-    if (__ballot(grow)) {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            float n = fmaxf(top[t], __shfl_xor(top[t], 16, 64));
-            n = fmaxf(n, __shfl_xor(n, 32, 64));
-            n = fmaxf(n, R.m[t]);
-            const float alpha = n == NEG_INF ? 1.0f : __builtin_amdgcn_exp2f(R.m[t] - n);
-            R.m[t] = n;
-            R.l[t] *= alpha;
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d) R.o[t][d] *= alpha;
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const float ref = R.m[t] == NEG_INF ? 0.0f : R.m[t];
-        u32x4_a pk;
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e], unit, -ref));
-            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][e + 1], unit, -ref));
-            const f32x2 two = {p0, p1};
-            pk[e >> 1] = __builtin_bit_cast(unsigned, __builtin_convertvector(two, bf16x2));
-        }
-        pb[t] = __builtin_bit_cast(bf16x8, pk);
-    }
+    const float unit = unit_of<CAP, BIAS>(p);
+    if (__ballot(block_top<D, RT>(R, s, unit, top))) block_grow<D, RT>(R, top);
+    block_weights<D, RT>(R, s, unit, pb);
 }
 
 // O^T += V^T P^T, and the sums of the same (rounded) weights
@@ -376,6 +384,56 @@ __device__ __forceinline__ void take_out_odd(Rows<D, RT>& R, u32x4_a (&vf)[D / 1
             vf[d][w] = ((v & 0x7f80u) == 0x7f80u ? 0u : v & 0xffffu) | ((v & 0x7f800000u) == 0x7f800000u ? 0u : v & 0xffff0000u);
         }
     }
+}
+
+// A 64-key tile whose pairs are all visible, for waves of 16 rows: its two blocks overlapped, one block's softmax (vector pipe) between
+// the other's matrix instructions (8 heads, 4096 tokens, D = 64: 78 against 86 us, causal 60 against 70; D = 128 109 against 111).  The weights are taken against the old reference maximum; a score that has outgrown it -- seldom -- sends the
+// block through block_grow and has its weights taken again.
+template <int NM, int NV>
+__device__ __forceinline__ void interleave() {           // NV vector instructions behind each of NM matrix instructions
+#pragma unroll
+    for (int i = 0; i < NM; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x402, NV, 0);
+    }
+}
+template <int D, int RT, bool CAP, bool BIAS>
+__device__ __forceinline__ void open_tile(const TextArgs& p, Rows<D, RT>& R, const char* smem, int k_at, int v_at, const float* win0) {
+    constexpr int NV = (CAP ? 8 : BIAS ? 5 : 4) * (D == 64 ? 2 : 1);
+    const float unit = unit_of<CAP, BIAS>(p);
+    bf16x8 k0[2][D / 32], k1[2][D / 32], p0[RT], p1[RT];
+    u32x4_a v0[D / 16], v1[D / 16];
+    float s0[RT][8], s1[RT][8], top[RT];
+    read_k<D>(smem, k_at, k0);
+    read_k<D>(smem, k_at + 64 * D, k1);
+    __builtin_amdgcn_sched_barrier(0);
+    block_qk<D, RT>(R, k0, s0);
+    __builtin_amdgcn_sched_barrier(0);
+    read_v<D>(smem, v_at, v0);
+    read_v<D>(smem, v_at + 64 * D, v1);
+    __builtin_amdgcn_sched_barrier(0);
+    block_qk<D, RT>(R, k1, s1);
+    cap_and_bias<D, RT, CAP, BIAS, false>(p, R, s0, win0);
+    bool grow = block_top<D, RT>(R, s0, unit, top);
+    block_weights<D, RT>(R, s0, unit, p0);
+    interleave<RT * 2 * (D / 32), NV>();
+    __builtin_amdgcn_sched_barrier(0);
+    if (__ballot(grow)) {
+        block_grow<D, RT>(R, top);
+        block_weights<D, RT>(R, s0, unit, p0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    block_pv<D, RT>(R, v0, p0);
+    cap_and_bias<D, RT, CAP, BIAS, false>(p, R, s1, win0 + 32);
+    grow = block_top<D, RT>(R, s1, unit, top);
+    block_weights<D, RT>(R, s1, unit, p1);
+    interleave<RT * (D / 16 + 1), NV>();
+    __builtin_amdgcn_sched_barrier(0);
+    if (__ballot(grow)) {
+        block_grow<D, RT>(R, top);
+        block_weights<D, RT>(R, s1, unit, p1);
+    }
+    block_pv<D, RT>(R, v1, p1);
 }
 
 // ---- which key tiles a workgroup visits ------------------------------------------------------------------------------------------
@@ -451,12 +509,13 @@ __device__ __forceinline__ void store_rows(const TextArgs& p, Rows<D, RT>& R, in
 }
 
 // ---- 128 or 64 rows per workgroup --------------------------------------------------------------------------------------------------
-// Bound by issue slots, not by memory or the matrix pipe: for one wave and 32-key block at D = 128 the matrix instructions take 544
-// clocks of about 1240, the softmax 98 vector and 74 scalar instructions; two waves of a SIMD cover each other in part (matrix pipe
-// busy 44 %).  1024 TFLOP/s at 28 / 4 heads, 8192 tokens, D = 128; 820 at 32 / 32 heads, 4096 tokens (333 us; cap 375 us, bias 353 us);
-// 755 at D = 64 (2 x 32 heads, 4096 tokens: 364 us).  At D = 64 the registers of three workgroups per CU are given room for: 490
-// against 554 us with a cap, 452 against 533 us with a bias, the plain forms alike.  Measured and not taken: a tile's two blocks
-// overlapped inside a wave (spills at D = 128, 407 against 364 us at D = 64), K fragments read a block ahead (slower on all sizes).
+// Bound by issue slots, not by memory or the matrix pipe: for one wave of 32 rows and a 32-key block at D = 128 the matrix instructions
+// take 544 clocks of about 1240, the softmax 98 vector and 74 scalar instructions; two waves of a SIMD cover each other in part (matrix
+// pipe busy 44 %).  1010 TFLOP/s at 28 / 4 heads, 8192 tokens, D = 128; 848 at 32 / 32 heads, 4096 tokens (324 us; cap 362 us, bias
+// 348 us); 780 at D = 64 (2 x 32 heads, 4096 tokens: 352 us).  At D = 64 the registers of three workgroups per CU are given room for:
+// 490 against 554 us with a cap, 452 against 533 us with a bias, 621 against 724 us with both (which costs 20 bytes of scratch).  Measured
+// and not taken: a tile's two blocks overlapped inside a wave of 32 rows (spills at D = 128, 407 against 364 us at D = 64; waves of 16
+// rows have the room), K fragments read a block ahead, and requests spread between the instructions (343 against 333 us).
 constexpr int TKEYS = 64;
 // floats per head of a tile's bias window: its 64 keys against every query of the row tile
 __host__ __device__ __forceinline__ int bias_window(int trows, int pack) { return TKEYS + (trows - 1) / pack + 2; }
@@ -503,7 +562,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
 
     const unsigned short* Kh = p.k + b * p.kb + (int64_t)hk * p.kh;
     const unsigned short* Vh = p.v + b * p.vb + (int64_t)hk * p.vh;
-    // a tile's requests in two parts (K, V), so that neither stands in front of the arithmetic as one burst.  A piece is 1 KiB = PER
+    // a tile's requests in two parts (K, V), so that neither stands in front of much arithmetic as one burst.  A piece is 1 KiB = PER
     // rows; of the swizzle's row bits two lie inside a piece and bit 3 is the same for a piece: i / 2 (D = 128: 4 rows), i (D = 64: 8).
     constexpr int PER = 64 / (D / 8), PIECES = TKEYS / PER / 4;
     const int vr = wave * PIECES * PER + lane / (D / 8), vc = (lane % (D / 8)) ^ swz<D>(lane / (D / 8));
@@ -572,11 +631,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
     }
     Rows<D, RT> R;                                     // (behind the first tile's requests: both are under way together)
     load_rows<D, RT>(p, R, seq, b, head0, tile * TROWS + wave * 16 * RT, q_last, win, lane);
-    // One loop over 32-key blocks, two to a tile (nested loops made the compiler keep a second copy of the accumulators).
+    // One loop over 32-key blocks, two to a tile (nested loops made the compiler keep a second copy of the accumulators); with 64 rows
+    // a tile that is visible as a whole takes both in one trip.
     int tn = -1, blk = 0;
     bool mine = false, masked = false;
     while (t >= 0) {
-        if (blk == 0) {
+        const bool first_trip = blk == 0;
+        if (first_trip) {
             tn = walk.next(lane, nlo, nhi);
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
@@ -584,14 +645,19 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
             if (tn >= 0) {
                 if (BIAS) fetch_bias(tn);
                 issue(tn, stage ^ 1, 0);
+                if (RT == 1) issue(tn, stage ^ 1, 1);
                 if (p.q_docs && wave == 0) issue_docs(tn, stage ^ 1);
             }
             const int first = t * TKEYS;
             mine = __builtin_amdgcn_readfirstlane((int)(first < R.lim_hi && (!p.q_docs || (dlo <= R.doc_hi && dhi >= R.doc_lo)))) != 0;
             masked = __builtin_amdgcn_readfirstlane((int)!(first + TKEYS <= R.lim_lo && (!p.q_docs || (dlo == dhi && R.doc_lo == R.doc_hi && dlo == R.doc_lo)))) != 0;
         }
-        if (mine) {
-            const int at = stage * 2 * OPER + blk * 32 * (2 * D), key0 = t * TKEYS + blk * 32;
+        const int at = stage * 2 * OPER + blk * 32 * (2 * D), key0 = t * TKEYS + blk * 32;
+        const float* const win0 = wins + stage * p.pack * win + blk * 32 + 8 * lq;
+        if (RT == 1 && mine && !masked && !(CAP && p.cap > CAP_WIDE)) {
+            open_tile<D, RT, CAP, BIAS>(p, R, smem, at + klane, at + OPER + vlane, win0);
+            blk = 1;
+        } else if (mine) {
             bf16x8 kf[2][D / 32], pb[RT];
             u32x4_a vf[D / 16];
             float s[RT][8];
@@ -603,13 +669,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
 #pragma unroll
                 for (int e = 0; e < 8; ++e) docs[e] = tile_docs[stage * 64 + blk * 32 + 8 * lq + e];
             }
-            block_softmax<D, RT, CAP, BIAS>(p, R, s, pb, key0, masked, docs, wins + stage * p.pack * win + blk * 32 + 8 * lq, lane);
+            __builtin_amdgcn_s_setprio(1);                // the vector pipe first: 4096 causal tokens 167 us, 173 without, 176 the other way round
+            block_softmax<D, RT, CAP, BIAS>(p, R, s, pb, key0, masked, docs, win0, lane);
+            __builtin_amdgcn_s_setprio(0);
             if (masked && any_odd<D>(vf)) take_out_odd<D, RT>(R, vf, pb);
             block_pv<D, RT>(R, vf, pb);
-        }
-        if (blk == 0) {
-            if (tn >= 0) issue(tn, stage ^ 1, 1);
         } else {
+            blk = 1;
+        }
+        if (RT == 2 && first_trip && tn >= 0) issue(tn, stage ^ 1, 1);
+        if (blk == 1) {
             if (BIAS && tn >= 0) write_bias(stage ^ 1);
             t = tn;
             dlo = nlo;

@@ -1,6 +1,6 @@
 """Static checks of the 4-bit GEMM kernels' and the text attention kernels' ISA (no GPU needed: hipcc cross-compiles): the hand-placed
-256 x 256 loop is what its generator writes, its accumulators are read before the compiler reuses them, and no kernel of the three
-sources uses scratch memory."""
+256 x 256 loop is what its generator writes, its accumulators are read before the compiler reuses them, and no kernel of the four
+sources uses scratch memory beyond what is stated."""
 import os
 import re
 import subprocess
@@ -40,7 +40,8 @@ def test_the_256_kernel(isa):
     found = list(_kernels(isa["ea_gemm.hip"], "gemm256_mxfp4_w4_kernel"))
     assert found
     for name, body in found:
-        assert not any("scratch_" in l for l in body) and not any("v_pk_" in l and "_f32" in l for l in body)
+        # (one address of the epilogue may wait out the loop in scratch memory)
+        assert sum("scratch_" in l for l in body) <= 2 and not any(re.search(r"v_pk_(add|mul|fma)_f32", l) for l in body)
         errors, _, _, n_loop_mfma, _ = _analyse(name, body)
         assert n_loop_mfma == [256], (name, n_loop_mfma)                       # two K tiles of 2 x 64 products
         assert not errors, "\n".join(errors[:10])
@@ -58,11 +59,13 @@ def test_generated_loop_is_the_committed_one(tmp_path):
     assert loop.count("v_mfma") == 256 and re.findall(r"s_c?branch\w* \w+", loop) == ["s_cbranch_scc0 9f"]
 
 
-@pytest.mark.parametrize("src,fragment,count", [("ea_gemm_mxfp4.hip", "gemm_mxfp4", None), ("ea_mxfp4.hip", "mxfp4", None), ("ea_attention_text.hip", "attention_text", 18)])
-def test_no_scratch_and_no_packed_fp32(isa, src, fragment, count):
+@pytest.mark.parametrize("src,fragment,count", [("ea_gemm_mxfp4.hip", "gemm_mxfp4", None), ("ea_mxfp4.hip", "mxfp4", None), ("ea_attention_text.hip", "attention_text", 28)])
+def test_scratch_and_no_packed_fp32(isa, src, fragment, count):
     found = list(_kernels(isa[src], fragment))
     assert found and (count is None or len(found) == count), [n for n, _ in found]
     for name, body in found:
-        bad = [l for l in body if "scratch_" in l or re.search(r"v_pk_(add|mul|fma)_f32", l)]
+        assert not [l for l in body if re.search(r"v_pk_(add|mul|fma)_f32", l)], name
         size = [int(l.split()[-1]) for l in body if ".amdhsa_private_segment_fixed_size" in l]
-        assert not bad and size == [0], (name, bad[:3], size)
+        # (three workgroups per CU at D = 64: a few registers of the bias forms spill, and that is faster than two)
+        allowed = 128 if "attention_text_kernelILi64E" in name and "ELb1EEE" in name else 0
+        assert len(size) == 1 and size[0] <= allowed, (name, size)
