@@ -669,9 +669,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
 #pragma unroll
                 for (int e = 0; e < 8; ++e) docs[e] = tile_docs[stage * 64 + blk * 32 + 8 * lq + e];
             }
-            __builtin_amdgcn_s_setprio(1);                // the vector pipe first: 4096 causal tokens 167 us, 173 without, 176 the other way round
+            if (D == 128) __builtin_amdgcn_s_setprio(1);  // the vector pipe first: 4096 causal tokens 167 us, 173 without, 176 the other way round (no gain at 64)
             block_softmax<D, RT, CAP, BIAS>(p, R, s, pb, key0, masked, docs, win0, lane);
-            __builtin_amdgcn_s_setprio(0);
+            if (D == 128) __builtin_amdgcn_s_setprio(0);
             if (masked && any_odd<D>(vf)) take_out_odd<D, RT>(R, vf, pb);
             block_pv<D, RT>(R, vf, pb);
         } else {
