@@ -12,6 +12,10 @@
 //   gemm_mxfp4_tile     256 x 128 .. 64 x 64 tiles through LDS, optionally K-split over workgroups (fp32 partial tiles in the caller's workspace,
 //                       joined in a fixed order by gemm_mxfp4_join)
 //   gemm256_mxfp4_w4    256 x 256 tiles with a hand-placed main loop (ea_gemm_mxfp4_w4.inc)
+//
+// What bounds it: the weight bytes for few rows (one token x 18944 x 3584: 11 us with its launch), the LDS fill of a CU for tiles up to
+// 128 x 128 (24 - 33 KB per K tile at 130 - 150 GB/s; 512 x 3584 x 18944 in 28 us = 2.5 PFLOP/s behind its quantisation), the matrix
+// pipe at the clock that the power budget leaves for the largest (8192^3 in 219 us = 5.0 PFLOP/s; ea_gemm_bf16 691 us).
 #include "ea_common.h"
 
 // ea_mxfp4.hip

@@ -8,7 +8,9 @@
 // tile at byte 2 g + j (the two that a lane of the product's matrix instructions needs are neighbours); elements >= K are zeros.
 // A 256-deep K tile of R rows is then one contiguous run for the product's LDS-DMA, and K needs no tail code there.
 //
-// Both directions are HBM-bound (2 + 17/32 bytes per element, no reuse).
+// Both directions are HBM-bound (2 + 17/32 bytes per element, no reuse): 13312 x 3584 in 18 us either way, 3584 x 18944 in 25 us = 6.6 -
+// 6.8 TB/s (a 2 GiB copy reaches 5.0; these fit the last-level cache in part).  Matrices of a few MB cost their launch.  Four rows per
+// thread keep four loads in flight; K tile by K tile per workgroup, not row by row, makes the code writes 4 KiB runs.
 #include "ea_common.h"
 
 namespace {
