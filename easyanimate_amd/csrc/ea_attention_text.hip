@@ -921,7 +921,7 @@ struct Plan {
     int64_t part_bytes, range_bytes;
 };
 
-Plan plan_of(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs) {
+Plan plan_of(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs, int causal) {
     Plan n;
     n.group = Hq / Hkv;
     n.pack = n.group < BIAS_PACK_MAX ? n.group : BIAS_PACK_MAX;
@@ -930,9 +930,11 @@ Plan plan_of(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs) {
     const int64_t sets = (int64_t)B * (Hq / n.pack);
     n.few = rows <= 16;
     n.key_tiles = (int)(((int64_t)Sk + TKEYS - 1) / TKEYS);
-    // 64 rows per workgroup where 128 would leave CUs without a second one (1024 causal tokens of 28 heads: 26 against 32 us; 2048 tokens,
-    // 448 workgroups of 128 rows: 79 us, 108 with 64)
-    n.rt = sets * ((rows + 127) / 128) <= 256 ? 1 : 2;
+    // 64 rows per workgroup while all of those run at once (two to a CU at D = 128, three at 64: 40 heads, 1024 tokens, D = 64, 640 of
+    // them: 27 against 32 us; 28 heads, 2048 tokens, D = 128: 108 us in 896 of them, 76 in 448 of 128 rows), and in causal order, where
+    // the longest workgroup sets the time, up to twice as many (32 heads, 2048 tokens, D = 64, 1024 of them: 36 against 46 us; 28 heads,
+    // D = 128, 896: 56 against 63; 40 heads, D = 64, 1280: 49 against 48)
+    n.rt = sets * ((rows + 127) / 128) <= (causal ? 512 : D == 64 ? 384 : 256) ? 1 : 2;
     n.row_tiles = n.few ? 1 : (int)((rows + 64 * n.rt - 1) / (64 * n.rt));
     // Split the keys while all workgroups still run at once (two to each of 256 CUs; 256 queries of 28 heads, 8192 keys: 64 us with 4
     // splits = 448 workgroups, 84 with 5) and a split keeps what pays for the join: 512 keys (128 queries, 4096 keys: 30 us; 38 with 256
@@ -996,7 +998,7 @@ bool sizes_ok(int B, int Hq, int Hkv, int Sq, int Sk, int D) {
 
 extern "C" int64_t ea_attention_text_workspace_bytes(int batch, int q_heads, int kv_heads, int q_len, int kv_len, int head_dim, int documents) {
     if (!sizes_ok(batch, q_heads, kv_heads, q_len, kv_len, head_dim) || q_len == 0 || kv_len == 0) return 0;
-    const Plan n = plan_of(batch, q_heads, kv_heads, q_len, kv_len, head_dim, documents);
+    const Plan n = plan_of(batch, q_heads, kv_heads, q_len, kv_len, head_dim, documents, 0);
     return n.part_bytes + n.range_bytes;
 }
 
@@ -1023,7 +1025,7 @@ extern "C" int ea_attention_text_bf16(const ea_bf16* q, const ea_bf16* k, const 
     EA_REQUIRE((batch == 1 || strides[9] >= (int64_t)q_heads * head_dim) && (q_len == 1 || strides[10] >= (int64_t)q_heads * head_dim),
                "ea_attention_text_bf16: rows of out overlap (strides %lld, %lld)", (long long)strides[9], (long long)strides[10]);
     EA_REQUIRE(strides[5] < (1 << 24) && strides[8] < (1 << 24), "ea_attention_text_bf16: row strides of k and v must be below 2^24 elements");
-    const Plan n = plan_of(batch, q_heads, kv_heads, q_len, kv_len, head_dim, q_docs != nullptr);
+    const Plan n = plan_of(batch, q_heads, kv_heads, q_len, kv_len, head_dim, q_docs != nullptr, causal);
     EA_REQUIRE(n.part_bytes + n.range_bytes == 0 ||
                    (workspace && workspace_bytes >= n.part_bytes + n.range_bytes && (uintptr_t)workspace % 16 == 0),
                "ea_attention_text_bf16: needs %lld bytes of 16-byte aligned workspace (ea_attention_text_workspace_bytes)",

@@ -83,7 +83,7 @@ def check(q, k, v, scale, kern=None, **kw):
     B, Hq, Sq, _ = q.shape
     pack = max(n for n in range(1, 9) if Hq // k.shape[1] % n == 0)
     if Sq * pack > 16:
-        reps = 256 // (B * Hq // pack * ((Sq * pack + 127) // 128)) + 1
+        reps = 512 // (B * Hq // pack * ((Sq * pack + 127) // 128)) + 1
         rep = lambda t: t.repeat(reps, *[1] * (t.dim() - 1))
         _lib.reset_counters()
         many = ops.attention_text(up(rep(q)), up(rep(k)), up(rep(v)), scale,
