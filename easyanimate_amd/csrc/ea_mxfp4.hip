@@ -33,8 +33,12 @@ __device__ __forceinline__ int scale_byte(int block) { return 2 * (block & 3) + 
 // 32, and a thread has ROWS_PER loads in flight.  Reads (writes) of 512 contiguous bytes per row, 128 x 32 contiguous code bytes;
 // neighbouring workgroups are neighbouring K tiles of the same rows.  The only division is the block index's (scalar, once).
 constexpr int ROWS_PER = 4, WG_ROWS = 8 * ROWS_PER;
+// 16 bytes on any even address: one access on this hardware
+typedef unsigned short u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
-// VEC: rows of x are 16-byte aligned and K % 8 == 0, so a thread's elements are one load, inside the row or outside it as a whole.
+// VEC: K % 8 == 0, so a thread's elements are one load, inside the row or outside it as a whole; otherwise the row's last ones are read
+// (written) one by one.
 // Row r of the output is row r % per of batch element r / per of x.
 template <bool VEC>
 __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const unsigned short* __restrict__ x, unsigned char* __restrict__ q,
@@ -51,9 +55,9 @@ __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const unsigned shor
         if (row < rows) {
             const int64_t b = per == rows ? 0 : row / per;
             const unsigned short* src = x + b * batch_stride + (row - b * per) * ld + k;
-            if (VEC) {
-                if (k < K) v[i] = *reinterpret_cast<const u16x8*>(src);
-            } else {
+            if (VEC ? k < K : k + 8 <= K) {
+                v[i] = *reinterpret_cast<const u16x8_any*>(src);
+            } else if (!VEC) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     if (k + e < K) v[i][e] = src[e];
@@ -108,8 +112,8 @@ __global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const unsigned ch
         w[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[i], scale, 3));
         if (row >= rows) continue;
         unsigned short* dst = y + row * (int64_t)K + k;
-        if (VEC) {
-            *reinterpret_cast<u32x4_q*>(dst) = w;
+        if (VEC || k + 8 <= K) {
+            *reinterpret_cast<u32x4_any*>(dst) = w;
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
@@ -132,7 +136,7 @@ int ea_mxfp4_quantize_launch(const unsigned short* x, unsigned char* codes, unsi
     const int kt = (int)(((int64_t)K + 255) / 256);
     dim3 grid;
     if (!grid_of(rows, kt, grid)) return EA_ERR_ARG;
-    if (K % 8 == 0 && ld % 8 == 0 && batch_stride % 8 == 0 && (((uintptr_t)x) & 15) == 0)
+    if (K % 8 == 0)
         hipLaunchKernelGGL(mxfp4_quantize_kernel<true>, grid, dim3(256), 0, st, x, codes, scales, rows, K, kt, ld, per, batch_stride);
     else
         hipLaunchKernelGGL(mxfp4_quantize_kernel<false>, grid, dim3(256), 0, st, x, codes, scales, rows, K, kt, ld, per, batch_stride);

@@ -145,8 +145,8 @@ int ea_gemm_bf16_w8(const ea_bf16* A, const uint8_t* W_fp8, const float* bias, e
  * e + 127; an element is the e2m1 code {0, 0.5, 1, 1.5, 2, 3, 4, 6} nearest to x / 2^e (ties to the even code, 6 at most) with its
  * sign.  A block holding an infinity or a NaN is byte 255 (NaN) with codes 0; a block of zeros byte 0.
  * Layout, K-blocked: codes [ceil(K/256)][rows][128] bytes (low nibble first), scales [ceil(K/256)][rows][8] bytes with the scale of
- * the tile's block 4 j + g (j < 2, g < 4) at byte 2 g + j; the elements past K of the last tile are zeros.  x: bf16 [rows, K], row stride ld >= K elements; K and ld need no alignment (multiples of 8 on
- * 16-byte aligned rows are read in 16-byte pieces).  codes 16-byte, scales 8-byte aligned.  Every byte of both outputs is written. */
+ * the tile's block 4 j + g (j < 2, g < 4) at byte 2 g + j; the elements past K of the last tile are zeros.  x: bf16 [rows, K], row stride ld >= K elements; x, K and ld
+ * need no alignment beyond their elements'.  codes 16-byte, scales 8-byte aligned.  Every byte of both outputs is written. */
 int ea_mxfp4_quantize_bf16(const ea_bf16* x, uint8_t* codes, uint8_t* scales, int64_t rows, int K, int64_t ld, void* stream);
 
 /* The stored values in bf16 (exact: code * 2^e has two significant bits): y bf16 [rows, K] contiguous. */
