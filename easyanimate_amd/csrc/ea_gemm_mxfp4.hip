@@ -9,12 +9,12 @@
 //
 //   gemm_mxfp4_skinny   few rows: 16 weight rows per workgroup, the K tiles dealt to its eight waves, operands straight from memory;
 //                       for M <= 16 the activations may still be bf16 (quantised on the way, same codes as ea_mxfp4_quantize_bf16)
-//   gemm_mxfp4_tile     256 x 128 .. 64 x 64 tiles through LDS, optionally K-split over workgroups (fp32 partial tiles in the caller's workspace,
+//   gemm_mxfp4_tile     256 x 128 .. 64 x 64 tiles through LDS, the small ones by two groups of waves, optionally K-split over workgroups (fp32 partial tiles in the caller's workspace,
 //                       joined in a fixed order by gemm_mxfp4_join)
 //   gemm256_mxfp4_w4    256 x 256 tiles with a hand-placed main loop (ea_gemm_mxfp4_w4.inc)
 //
 // What bounds it: the weight bytes for few rows (one token x 18944 x 3584: 11 us with its launch), the LDS fill of a CU for tiles up to
-// 128 x 128 (24 - 33 KB per K tile at 130 - 150 GB/s; 512 x 3584 x 18944 in 28 us = 2.5 PFLOP/s behind its quantisation), the matrix
+// 128 x 128 (24 - 33 KB per K tile at 130 - 150 GB/s; 512 x 3584 x 18944 in 33 us = 2.1 PFLOP/s with its weights from memory), the matrix
 // pipe at the clock that the power budget leaves for the largest (8192^3 in 219 us = 5.0 PFLOP/s; ea_gemm_bf16 691 us).
 #include "ea_common.h"
 
@@ -213,8 +213,13 @@ __device__ __forceinline__ bool mx_tile_of_block(const MxArgs& p, int& tm, int& 
 // BM x BN tiles, WM x WN waves, NS stages of one K tile each filled by LDS-DMA up to NS - 1 tiles ahead: rows of 128 bytes with the
 // 16-byte chunks XOR-swizzled by row & 7 (eight consecutive rows of a fragment read hit eight different 16-byte columns), and behind
 // them the tile's scale bytes.  One barrier per tile; the wait in front of it leaves the younger tiles in flight.
-template <int BM, int BN, int WM, int WN, int NS, int EPI, bool SPLIT>
-__global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) void gemm_mxfp4_tile_kernel(MxArgs p) {
+//
+// KG = 2: two such groups of waves, which take the K tiles in turn (each its own stages) and join their sums through LDS: where tiles are
+// few, a CU's four SIMDs have two waves each to cover what a K tile's chain of LDS reads, products and barrier leaves idle (128 x 64
+// tiles, 512 x 3584 x 18944: 33 against 38 us; 64 x 64, 128 x 4096 x 11008: 12.4 against 15.1; no size slower).  128 x 128 tiles get the
+// same from eight waves of 32 x 64 (1024 x 4096 x 4096: 15.2 us, four waves 15.8, two groups with two stages 16.7).
+template <int BM, int BN, int WM, int WN, int NS, int KG, int EPI, bool SPLIT>
+__global__ __launch_bounds__(64 * WM * WN * KG, BM * BN / (WM * WN) > 4096 ? 1 : 2) void gemm_mxfp4_tile_kernel(MxArgs p) {
     constexpr int WAVES = WM * WN;
     constexpr int TI = BM / (16 * WM), TJ = BN / (16 * WN);     // 16 x 16 MFMA tiles of a wave
     constexpr int PA = BM / (8 * WAVES), PW = BN / (8 * WAVES); // 1 KiB pieces of a wave, per operand
@@ -222,9 +227,10 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) v
     constexpr int OPER_A = BM * 128, OPER_W = BN * 128, STAGE = OPER_A + OPER_W + SRUNS * WAVES * 256;
     constexpr int LOADS = PA + PW + SRUNS;                      // per wave and tile
     static_assert((NS - 1) * LOADS < 64, "the counted wait has six bits");
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    extern __shared__ __attribute__((aligned(16))) char smem_all[];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave_all = __builtin_amdgcn_readfirstlane(tid >> 6), kg = wave_all / WAVES, wave = wave_all % WAVES;
+    char* const smem = smem_all + kg * (NS * STAGE);
     const int wr = wave / WN, wc = wave % WN, lr = lane & 15, g = lane >> 4;
     int tm, tn;
     if (!mx_tile_of_block(p, tm, tn)) return;
@@ -232,6 +238,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) v
     const int row0 = tm * BM, col0 = tn * BN;
     const int t0 = SPLIT ? (int)((int64_t)p.kt * blockIdx.z / p.splits) : 0;
     const int t1 = SPLIT ? (int)((int64_t)p.kt * (blockIdx.z + 1) / p.splits) : p.kt;
+    const int own = (t1 - t0 - kg + KG - 1) / KG;      // K tiles t0 + kg, + KG, ..: this group's; the other group's may be one more
     const int64_t a_tile = p.a_rows * 128, w_tile = (int64_t)p.N * 128;
 
     // byte offsets inside the tile's rows of each operand (rows past the end read the last one again)
@@ -255,10 +262,10 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) v
         const int last = (run < BM / 32 ? p.M - row0 : p.N - col0) - 1;
         sv[n] = (r < last ? r : last) * 8 + (lane & 1) * 4;
     }
-    const unsigned char* pa = p.A + t0 * a_tile + ((int64_t)b * p.M + row0) * 128;
-    const unsigned char* pw = p.W + t0 * w_tile + (int64_t)col0 * 128;
-    const unsigned char* psa = p.As + (t0 * p.a_rows + (int64_t)b * p.M + row0) * 8;
-    const unsigned char* psw = p.Ws + ((int64_t)t0 * p.N + col0) * 8;
+    const unsigned char* pa = p.A + (t0 + kg) * a_tile + ((int64_t)b * p.M + row0) * 128;
+    const unsigned char* pw = p.W + (t0 + kg) * w_tile + (int64_t)col0 * 128;
+    const unsigned char* psa = p.As + ((t0 + kg) * p.a_rows + (int64_t)b * p.M + row0) * 8;
+    const unsigned char* psw = p.Ws + ((int64_t)(t0 + kg) * p.N + col0) * 8;
     f32x4 acc[TI][TJ];
 #pragma unroll
     for (int i = 0; i < TI; ++i)
@@ -276,10 +283,10 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) v
         }
     };
     auto advance = [&]() {
-        pa += a_tile;
-        pw += w_tile;
-        psa += p.a_rows * 8;
-        psw += (int64_t)p.N * 8;
+        pa += KG * a_tile;
+        pw += KG * w_tile;
+        psa += KG * p.a_rows * 8;
+        psw += KG * (int64_t)p.N * 8;
     };
     // The two MFMA halves of a K tile carry everything else between their MFMAs, one instruction at a time, so that neither the LDS
     // reads nor the requests (a burst of them holds the wave until the memory pipe has taken them) stand in front of the matrix pipe:
@@ -300,15 +307,15 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) v
         if (f < TJ) swn[f < TJ ? f : 0] = *reinterpret_cast<const unsigned short*>(base + sw_off + f * 128);
         else san[f >= TJ ? f - TJ : 0] = *reinterpret_cast<const unsigned short*>(base + sa_off + (f - TJ) * 128);
     };
-    const int n = t1 - t0;
+    const int n = (t1 - t0 + KG - 1) / KG;             // trips: the last of one group may be empty
 #pragma unroll
     for (int t = 0; t < NS - 1; ++t) {
 #pragma unroll
-        for (int d = 0; d < LOADS; ++d) request(d, t, t < n);
+        for (int d = 0; d < LOADS; ++d) request(d, t, t < own);
         advance();
     }
 #pragma unroll
-    for (int d = 0; d < LA; ++d) request(d, NS - 1, NS - 1 < n);
+    for (int d = 0; d < LA; ++d) request(d, NS - 1, NS - 1 < own);
     // this wave's requests of the first tile have landed, then everybody's
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * LOADS + LA) : "memory");
     __builtin_amdgcn_s_barrier();
@@ -321,9 +328,9 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) v
     int st = 0;
     for (int t = 0; t < n; ++t) {
 #pragma unroll
-        for (int i = 0; i < TI; ++i) sa[i] = san[i];
+        for (int i = 0; i < TI; ++i) sa[i] = KG == 1 || t < own ? san[i] : 0;       // (scale bytes 0: whatever the codes, products below 2^-240)
 #pragma unroll
-        for (int j = 0; j < TJ; ++j) sw[j] = swn[j];
+        for (int j = 0; j < TJ; ++j) sw[j] = KG == 1 || t < own ? swn[j] : 0;
         const int prev = st == 0 ? NS - 1 : st - 1;                  // stage of tile t + NS - 1
 #pragma unroll
         for (int m = 0; m < SLOTS; ++m) {
@@ -332,7 +339,7 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) v
             for (int f = 0; f < F0; ++f)
                 if (f >= m * F0 / SLOTS && f < (m + 1) * F0 / SLOTS) {
                     if (f < FR) read_frag(f, smem + st * STAGE, ch1, a1, w1);
-                    else request(LA + f - FR, prev, t + NS - 1 < n);
+                    else request(LA + f - FR, prev, t + NS - 1 < own);
                 }
             acc[m % TI][m / TI] = mfma_mx<0>(w0[m / TI], sw[m / TI], a0[m % TI], sa[m % TI], acc[m % TI][m / TI]);
             __builtin_amdgcn_sched_barrier(0);
@@ -351,17 +358,39 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) v
                 if (f >= m * F1 / SLOTS && f < (m + 1) * F1 / SLOTS) {      // (behind the last tile: an old stage's bytes, not used)
                     if (f < FR) read_scale(f, smem + st * STAGE);
                     else if (f < 2 * FR) read_frag(f - FR, smem + st * STAGE, ch0, a0, w0);
-                    else request(f - 2 * FR, cur, t + NS < n);
+                    else request(f - 2 * FR, cur, t + NS < own);
                 }
             acc[m % TI][m / TI] = mfma_mx<1>(w1[m / TI], sw[m / TI], a1[m % TI], sa[m % TI], acc[m % TI][m / TI]);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
+    // join: each group takes half of the tile's row blocks, the other group's sums for them come through LDS
+    constexpr int TK = TI / KG;
+    if (KG == 2) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");      // (no request may land behind this)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        f32x4* const box = reinterpret_cast<f32x4*>(smem_all) + wave * (TI * TJ * 64) + lane;
+#pragma unroll
+        for (int i = 0; i < TI; ++i)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j)
+                if (i / TK != kg) box[(i * TJ + j) * 64] = acc[i][j];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TK; ++i)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j) {
+                const f32x4 mine = kg ? acc[i + (KG - 1) * TK][j] : acc[i][j];
+                acc[i][j] = mine + box[((i + kg * TK) * TJ + j) * 64];
+            }
+    }
+    const int row_out = row0 + wr * (BM / WM) + (KG == 2 ? kg * TK * 16 : 0);
     const int n00 = col0 + wc * (BN / WN) + g * 4;
     if (SPLIT) {
 #pragma unroll
-        for (int i = 0; i < TI; ++i) {
-            const int m = row0 + wr * (BM / WM) + i * 16 + lr;
+        for (int i = 0; i < TK; ++i) {
+            const int m = row_out + i * 16 + lr;
 #pragma unroll
             for (int j = 0; j < TJ; ++j)
                 if (m < p.M && n00 + j * 16 < p.N)
@@ -378,8 +407,8 @@ __global__ __launch_bounds__(64 * WM * WN, BM * BN / (WM * WN) > 4096 ? 1 : 2) v
         gv[j] = mx_gate<EPI>(p, b, nc[j]);
     }
 #pragma unroll
-    for (int i = 0; i < TI; ++i) {
-        const int m = row0 + wr * (BM / WM) + i * 16 + lr, mc = m < p.M ? m : p.M - 1;
+    for (int i = 0; i < TK; ++i) {
+        const int m = row_out + i * 16 + lr, mc = m < p.M ? m : p.M - 1;
         u16x4_m rr[TJ];
 #pragma unroll
         for (int j = 0; j < TJ; ++j) rr[j] = mx_res<EPI>(p, b, mc, nc[j]);
@@ -412,11 +441,11 @@ struct MxPlan {
 };
 int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
-// Tiles and what a K tile of one costs a CU, in microseconds, between running alone and with the whole chip busy (256 x 128: 0.58 and
-// 0.92; 128 x 128: 0.44 and 0.58; 128 x 64: 0.33 and 0.30; 64 x 64: 0.25 and 0.19).  A grid takes ceil(tiles / 256 CUs) of them per
-// K tile; the cheapest grid is taken: 256 x 18944 x 3584 runs in 20 us on 148 of the largest tiles and in 24 - 28 us on the others, 512
-// x 3584 x 18944 in 32 us on 224 tiles of 128 x 64 and in 36 - 39 us on the others, 1024 x 4096 x 4096 in 15 us on 256 of 128 x 128 and
-// in 16 - 19 us on the others.
+// Tiles and what a K tile of one costs a CU, in microseconds, between running alone and with the whole chip busy.  A grid takes
+// ceil(tiles / 256 CUs) of them per K tile; the cheapest grid is taken: 256 x 18944 x 3584 runs in 22 us on 148 of the largest tiles and
+// in 28 - 36 us on the others, 512 x 3584 x 18944 in 33 us on 224 tiles of 128 x 64 and in 35 - 46 us on the others, 1024 x 4096 x 4096 in
+// 15 us on 256 of 128 x 128 and in 18 - 25 us on the others, 256 x 4096 x 4096 in 7.4 us on 256 of 64 x 64 and in 9 - 17 us on the others
+// (weights from memory).
 struct MxTile { int bm, bn; float us; };
 constexpr float MX_W4_US = 1.2f;         // 256 x 256 tiles (ea_gemm_mxfp4_w4.inc)
 constexpr MxTile MX_TILES[4] = {{256, 128, 0.75f}, {128, 128, 0.52f}, {128, 64, 0.33f}, {64, 64, 0.22f}};
@@ -453,17 +482,17 @@ MxPlan mx_plan(int batch, int M, int N, int K, bool from_bf16, bool vec) {
     return n;
 }
 
-template <int BM, int BN, int WM, int WN, int NS, int EPI, bool SPLIT>
+template <int BM, int BN, int WM, int WN, int NS, int KG, int EPI, bool SPLIT>
 int mx_launch_tile(const MxArgs& p, hipStream_t st) {
-    constexpr int WAVES = WM * WN, LDS = NS * ((BM + BN) * 128 + ((BM + BN) / 32 + WAVES - 1) / WAVES * WAVES * 256);
-    const auto kern = gemm_mxfp4_tile_kernel<BM, BN, WM, WN, NS, EPI, SPLIT>;
+    constexpr int WAVES = WM * WN, LDS = KG * NS * ((BM + BN) * 128 + ((BM + BN) / 32 + WAVES - 1) / WAVES * WAVES * 256);
+    const auto kern = gemm_mxfp4_tile_kernel<BM, BN, WM, WN, NS, KG, EPI, SPLIT>;
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (e != hipSuccess) {
         ea_set_error("ea_gemm_mxfp4: %d bytes of LDS: %s", LDS, hipGetErrorString(e));
         return (int)e;
     }
     const dim3 grid((unsigned)((p.tiles_m * p.tiles_n + 7) / 8 * 8), (unsigned)p.batch, (unsigned)p.splits);
-    hipLaunchKernelGGL(kern, grid, dim3(64 * WAVES), LDS, st, p);
+    hipLaunchKernelGGL(kern, grid, dim3(64 * WAVES * KG), LDS, st, p);
     return EA_OK;
 }
 
@@ -491,19 +520,19 @@ int mx_launch(MxArgs& p, const MxPlan& n, hipStream_t st) {
     switch (n.cfg) {
         case 0:
             ea_count(split ? "gemm_mxfp4_256x128_split" : "gemm_mxfp4_256x128");
-            rc = split ? mx_launch_tile<256, 128, 4, 2, 3, EPI, true>(p, st) : mx_launch_tile<256, 128, 4, 2, 3, EPI, false>(p, st);
+            rc = split ? mx_launch_tile<256, 128, 4, 2, 3, 1, EPI, true>(p, st) : mx_launch_tile<256, 128, 4, 2, 3, 1, EPI, false>(p, st);
             break;
         case 1:
             ea_count(split ? "gemm_mxfp4_128x128_split" : "gemm_mxfp4_128x128");
-            rc = split ? mx_launch_tile<128, 128, 2, 2, 3, EPI, true>(p, st) : mx_launch_tile<128, 128, 2, 2, 3, EPI, false>(p, st);
+            rc = split ? mx_launch_tile<128, 128, 4, 2, 4, 1, EPI, true>(p, st) : mx_launch_tile<128, 128, 4, 2, 4, 1, EPI, false>(p, st);
             break;
         case 2:
             ea_count(split ? "gemm_mxfp4_128x64_split" : "gemm_mxfp4_128x64");
-            rc = split ? mx_launch_tile<128, 64, 2, 2, 3, EPI, true>(p, st) : mx_launch_tile<128, 64, 2, 2, 3, EPI, false>(p, st);
+            rc = split ? mx_launch_tile<128, 64, 2, 2, 3, 2, EPI, true>(p, st) : mx_launch_tile<128, 64, 2, 2, 3, 2, EPI, false>(p, st);
             break;
         default:
             ea_count(split ? "gemm_mxfp4_64x64_split" : "gemm_mxfp4_64x64");
-            rc = split ? mx_launch_tile<64, 64, 2, 2, 4, EPI, true>(p, st) : mx_launch_tile<64, 64, 2, 2, 4, EPI, false>(p, st);
+            rc = split ? mx_launch_tile<64, 64, 2, 2, 4, 2, EPI, true>(p, st) : mx_launch_tile<64, 64, 2, 2, 4, 2, EPI, false>(p, st);
     }
     if (rc == EA_OK && split) {
         const int64_t t = (int64_t)p.batch * p.M * (p.N / 4);
