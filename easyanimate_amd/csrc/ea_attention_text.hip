@@ -511,9 +511,9 @@ __device__ __forceinline__ void store_rows(const TextArgs& p, Rows<D, RT>& R, in
 // ---- 128 or 64 rows per workgroup --------------------------------------------------------------------------------------------------
 // Bound by issue slots, not by memory or the matrix pipe: for one wave of 32 rows and a 32-key block at D = 128 the matrix instructions
 // take 544 clocks of about 1240, the softmax 98 vector and 74 scalar instructions; two waves of a SIMD cover each other in part (matrix
-// pipe busy 44 %).  1010 TFLOP/s at 28 / 4 heads, 8192 tokens, D = 128; 848 at 32 / 32 heads, 4096 tokens (324 us; cap 362 us, bias
-// 348 us); 780 at D = 64 (2 x 32 heads, 4096 tokens: 352 us).  At D = 64 the registers of three workgroups per CU are given room for:
-// 490 against 554 us with a cap, 452 against 533 us with a bias, 621 against 724 us with both (which costs 20 bytes of scratch).  Measured
+// pipe busy 44 %).  1000 TFLOP/s at 28 / 4 heads, 8192 tokens, D = 128; 851 at 32 / 32 heads, 4096 tokens (323 us; cap 365 us, bias
+// 351 us); 790 at D = 64 (2 x 32 heads, 4096 tokens: 350 us).  At D = 64 the registers of three workgroups per CU are given room for:
+// 480 against 554 us with a cap, 448 against 533 us with a bias, 621 against 724 us with both (which costs 20 bytes of scratch).  Measured
 // and not taken: a tile's two blocks overlapped inside a wave of 32 rows (spills at D = 128, 407 against 364 us at D = 64; waves of 16
 // rows have the room), K fragments read a block ahead, and requests spread between the instructions (343 against 333 us).
 constexpr int TKEYS = 64;
@@ -931,10 +931,10 @@ Plan plan_of(int B, int Hq, int Hkv, int Sq, int Sk, int D, int docs, int causal
     n.few = rows <= 16;
     n.key_tiles = (int)(((int64_t)Sk + TKEYS - 1) / TKEYS);
     // 64 rows per workgroup while all of those run at once (two to a CU at D = 128, three at 64: 40 heads, 1024 tokens, D = 64, 640 of
-    // them: 27 against 32 us; 28 heads, 2048 tokens, D = 128: 108 us in 896 of them, 76 in 448 of 128 rows), and in causal order, where
-    // the longest workgroup sets the time, up to twice as many (32 heads, 2048 tokens, D = 64, 1024 of them: 36 against 46 us; 28 heads,
-    // D = 128, 896: 56 against 63; 40 heads, D = 64, 1280: 49 against 48)
-    n.rt = sets * ((rows + 127) / 128) <= (causal ? 512 : D == 64 ? 384 : 256) ? 1 : 2;
+    // them: 27 against 32 us; 28 heads, 2048 tokens, D = 128: 108 us in 896 of them, 76 in 448 of 128 rows), and in causal order over 16 or
+    // more key tiles, where the longest workgroup sets the time, up to 1024 of them (32 heads, 2048 tokens, D = 64: 36 against 46 us; 28
+    // heads, D = 128, 896: 56 against 63; 40 heads, D = 64, 1280: 49 against 48; 128 heads, 512 tokens, D = 64: 17.7 against 16.5)
+    n.rt = sets * ((rows + 127) / 128) <= (causal && n.key_tiles >= 16 ? 512 : D == 64 ? 384 : 256) ? 1 : 2;
     n.row_tiles = n.few ? 1 : (int)((rows + 64 * n.rt - 1) / (64 * n.rt));
     // Split the keys while all workgroups still run at once (two to each of 256 CUs; 256 queries of 28 heads, 8192 keys: 64 us with 4
     // splits = 448 workgroups, 84 with 5) and a split keeps what pays for the join: 512 keys (128 queries, 4096 keys: 30 us; 38 with 256

@@ -13,7 +13,7 @@
 //                       joined in a fixed order by gemm_mxfp4_join)
 //   gemm256_mxfp4_w4    256 x 256 tiles with a hand-placed main loop (ea_gemm_mxfp4_w4.inc)
 //
-// What bounds it: the weight bytes for few rows (one token x 18944 x 3584: 11 us with its launch), the LDS fill of a CU for tiles up to
+// What bounds it: the weight bytes for few rows (one token x 3584 x 3584: 5.3 us, x 18944 x 3584: 10), the LDS fill of a CU for tiles up to
 // 128 x 128 (24 - 33 KB per K tile at 130 - 150 GB/s; 512 x 3584 x 18944 in 33 us = 2.1 PFLOP/s with its weights from memory), the matrix
 // pipe at the clock that the power budget leaves for the largest (8192^3 in 219 us = 5.0 PFLOP/s; ea_gemm_bf16 691 us).
 #include "ea_common.h"
