@@ -485,7 +485,7 @@ __device__ __forceinline__ void store_rows(const TextArgs& p, Rows<D, RT>& R, in
         const float l = R.l[t][0];
         const int in = row0 + t * 16 + lr, qi = in / p.pack, hg = in - qi * p.pack;
         if (qi >= p.Sq) continue;
-        if (p.splits == 1) {
+        if (RT == 2 || p.splits == 1) {                  // (the 128-row tiles are never split)
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             unsigned short* dst = p.out + b * p.ob + (int64_t)qi * p.os + (int64_t)(head0 + hg) * D + lq * 4;
 #pragma unroll
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
     const int set_all = blockIdx.x % (nsets * p.B), tile = p.row_tiles - 1 - blockIdx.x / (nsets * p.B);
     const int b = set_all / nsets, set = set_all % nsets;
     const int head0 = set * p.pack, hk = head0 / p.group;
-    const int split = blockIdx.y;
+    const int split = RT == 2 ? 0 : blockIdx.y, splits = RT == 2 ? 1 : p.splits;
     const int rows = p.Sq * p.pack;
     const int q_first = tile * TROWS / p.pack;
     const int q_last = min((tile * TROWS + TROWS - 1) / p.pack, p.Sq - 1);
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attention_text_kernel(Te
         walk.dhi = __builtin_amdgcn_readfirstlane(wave_max(hi));
         walk.range = p.doc_range + (int64_t)b * p.key_tiles * 2;
     }
-    walk.start((int)((int64_t)nt * split / p.splits), (int)((int64_t)nt * (split + 1) / p.splits), lane);
+    walk.start((int)((int64_t)nt * split / splits), (int)((int64_t)nt * (split + 1) / splits), lane);
 
     const unsigned short* Kh = p.k + b * p.kb + (int64_t)hk * p.kh;
     const unsigned short* Vh = p.v + b * p.vb + (int64_t)hk * p.vh;

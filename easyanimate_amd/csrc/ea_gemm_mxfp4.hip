@@ -475,9 +475,10 @@ MxPlan mx_plan(int batch, int M, int N, int K, bool from_bf16, bool vec) {
     }
     n.w4 = (double)((mx_tiles({256, 256, 0}, batch, M, N) + 255) / 256) * MX_W4_US < best;
     if (n.w4) return n;
-    // few tiles and a long K: split it while a split keeps 24 K tiles (6 us; joining two splits costs about 4)
+    // few tiles and a long K: split it while a split keeps 24 K tiles (6 us; joining two splits costs about 4).  (A larger tile is only
+    // chosen when there are more than 256 of the next smaller one, so more than 128 of its own.)
     const int64_t tiles = mx_tiles(MX_TILES[n.cfg], batch, M, N);
-    while (tiles * n.splits * 2 <= 256 && kt / (n.splits * 2) >= 24 && n.splits < 16) n.splits *= 2;
+    while (n.cfg == 3 && tiles * n.splits * 2 <= 256 && kt / (n.splits * 2) >= 24 && n.splits < 16) n.splits *= 2;
     if (n.splits > 1) n.part_bytes = (int64_t)n.splits * batch * M * N * 4;
     return n;
 }
@@ -519,16 +520,16 @@ int mx_launch(MxArgs& p, const MxPlan& n, hipStream_t st) {
     const bool split = n.splits > 1;
     switch (n.cfg) {
         case 0:
-            ea_count(split ? "gemm_mxfp4_256x128_split" : "gemm_mxfp4_256x128");
-            rc = split ? mx_launch_tile<256, 128, 4, 2, 3, 1, EPI, true>(p, st) : mx_launch_tile<256, 128, 4, 2, 3, 1, EPI, false>(p, st);
+            ea_count("gemm_mxfp4_256x128");
+            rc = mx_launch_tile<256, 128, 4, 2, 3, 1, EPI, false>(p, st);
             break;
         case 1:
-            ea_count(split ? "gemm_mxfp4_128x128_split" : "gemm_mxfp4_128x128");
-            rc = split ? mx_launch_tile<128, 128, 4, 2, 4, 1, EPI, true>(p, st) : mx_launch_tile<128, 128, 4, 2, 4, 1, EPI, false>(p, st);
+            ea_count("gemm_mxfp4_128x128");
+            rc = mx_launch_tile<128, 128, 4, 2, 4, 1, EPI, false>(p, st);
             break;
         case 2:
-            ea_count(split ? "gemm_mxfp4_128x64_split" : "gemm_mxfp4_128x64");
-            rc = split ? mx_launch_tile<128, 64, 2, 2, 3, 2, EPI, true>(p, st) : mx_launch_tile<128, 64, 2, 2, 3, 2, EPI, false>(p, st);
+            ea_count("gemm_mxfp4_128x64");
+            rc = mx_launch_tile<128, 64, 2, 2, 3, 2, EPI, false>(p, st);
             break;
         default:
             ea_count(split ? "gemm_mxfp4_64x64_split" : "gemm_mxfp4_64x64");
