@@ -17,6 +17,9 @@ def pytest_collection_modifyitems(items):
     for it in items:
         if it.nodeid.endswith("test_fence_gpu.py::test_fence_positive_control"):
             it.add_marker(pytest.mark.skip(reason="faults the GPU on purpose; no test run may"))
+        # an empty reference folder is no reference: the scripts' surface then comes from its committed copy
+        if it.nodeid.startswith("tests/test_dropin_scripts_cpu.py") and not os.path.exists(os.path.join(it.module.REF, it.module.SCRIPTS[0])):
+            it.module.REF = ""
 
 
 @pytest.fixture(scope="session")
