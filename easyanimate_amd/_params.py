@@ -66,6 +66,8 @@ class weights_frozen:
 
     def __enter__(self):
         global _frozen
+        if _frozen == 0:
+            drop_tag("mxfp4")        # (what an earlier region laid out may be older than a `.data` write since)
         _frozen += 1
         return self
 
@@ -115,11 +117,15 @@ def bf16_weight(p, k_pad: int | None = None):
 
 
 def mxfp4_weight(p):
-    """The microscaled 4-bit storage (ops.Mxfp4, 17 / 32 byte per weight) of a Linear weight [N, K], cached like every derived weight:
-    laid out again after load_state_dict, in-place writes or a move; writes through `.data` need invalidate_weight_cache(), which the
-    pipelines call at the start of each run."""
+    """The microscaled 4-bit storage (ops.Mxfp4, 17 / 32 byte per weight) of a Linear weight [N, K].  Kept inside a weights_frozen()
+    region only: outside of it laid out anew on every use, so that a write through `.data` is seen too (like kblocked_weight; 2.5 bytes
+    of traffic per weight, 25 us for 3584 x 18944)."""
     from . import ops
-    return derived(p, "mxfp4", lambda t: ops.mxfp4_quantize(t.to(torch.bfloat16)))
+    make = lambda t: ops.mxfp4_quantize(t.to(torch.bfloat16))
+    if not frozen():
+        with torch.no_grad():
+            return make(p.detach())
+    return derived(p, "mxfp4", make)
 
 
 def kblocked_weight(p):

@@ -55,7 +55,7 @@ class Qwen2VLTextEncoderHIP(nn.Module):
         """padded_positions: the rotary position of the right-PADDED slots (real tokens are 0 .. n-1 either way; the DiT consumes
         the padded rows too, transformer3d.py:1502).  "arange" = transformers 5.x (the installed version: text-only prompts get
         the text model's own arange(S)); "cumsum_fill1" = transformers 4.46 - 4.5x (get_rope_index: cumsum(mask) - 1, padding -> 1).
-        weights: "bf16", or "mxfp4" for 4-bit Linear layers (laid out at the first call)."""
+        weights: "bf16", or "mxfp4" for 4-bit Linear layers (laid out per call, or once inside _params.weights_frozen())."""
         super().__init__()
         if padded_positions not in ("arange", "cumsum_fill1"):
             raise ValueError(f"padded_positions must be 'arange' or 'cumsum_fill1', not {padded_positions!r}")

@@ -112,6 +112,7 @@ def test_layers_stage_by_stage(case, monkeypatch):
 
 
 def test_a_changed_weight_is_laid_out_again():
+    from easyanimate_amd._params import weights_frozen
     from easyanimate_amd.text_encoder import Qwen2VLTextEncoderHIP
     c = CASES["hd64"]
     hf = _qwen(c["hidden"], c["heads"], c["kv_heads"], c["inter"], c["layers"]).to(torch.bfloat16).to(DEV)
@@ -124,6 +125,14 @@ def test_a_changed_weight_is_laid_out_again():
     after = run(enc)
     assert not torch.equal(before, after)
     assert torch.equal(after, run(Qwen2VLTextEncoderHIP(hf, weights="mxfp4")))
+    enc._text[0].layers[1].mlp.up_proj.weight.data.mul_(-1.0)               # no version counter sees this one
+    third = run(enc)
+    assert not torch.equal(third, after)
+    with weights_frozen():                                                  # laid out once for the region
+        assert torch.equal(run(enc), third) and torch.equal(run(enc), third)
+    enc._text[0].layers[1].mlp.up_proj.weight.data.mul_(-1.0)
+    with weights_frozen():
+        assert torch.equal(run(enc), after)
 
 
 def test_pipeline_slot():
