@@ -830,11 +830,9 @@ __global__ __launch_bounds__(256, 2) void attention_text_few_kernel(TextArgs p) 
     store_rows<D, 1>(p, R, b, head0, (int64_t)set_all * rows, split, (int64_t)p.B * nsets * rows, 0, lane);
 }
 
-// One workgroup per row: the splits' weights first (one thread each), then 256 / D threads per output element over the splits, each
-// taking every (256 / D)-th, and their sums in a fixed order.
+// ---- the splits' partial results joined, in the order of the splits: up to 12 splits D / 4 threads per row (8400 rows, 3 splits: 24 us
+// with the attention, 31 with a workgroup per row), else a workgroup per row (448 rows, 64 splits: 23 us, 31 the other way)
 constexpr int MAX_SPLITS = 256;
-// Up to 12 splits D / 4 threads per row: 8400 rows, 3 splits, 24 us altogether, 31 with a workgroup per row (448 rows, 64 splits: 31
-// against 23).
 template <int D>
 __device__ __forceinline__ unsigned short* out_row_of(const TextArgs& p, const int64_t row) {
     // row = ((b * sets + set) * Sq + query) * pack + head of the set
@@ -870,6 +868,8 @@ __global__ __launch_bounds__(256) void attention_text_join_rows_kernel(TextArgs 
     *reinterpret_cast<bf16x4*>(out_row_of<D>(p, row) + d) = v;
 }
 
+// The splits' weights first (one thread each), then 256 / D threads per output element, each taking every (256 / D)-th split, and their
+// sums in a fixed order.
 template <int D>
 __global__ __launch_bounds__(256) void attention_text_join_kernel(TextArgs p) {
     constexpr int PARTS = 256 / D;
