@@ -336,18 +336,24 @@ def gemm_mxfp4(A: Union[torch.Tensor, Mxfp4], W: Mxfp4, bias: Optional[torch.Ten
     if packed:
         B, M, ak, squeeze, dev = 1, A.rows, A.k, True, A.codes.device
     else:
-        _chk(A, _BF16, "A")
-        squeeze, dev = A.dim() == 2, A.device
+        if A.dtype != _BF16:
+            _chk(A, _BF16, "A")
+        sh, dev = A.shape, A.device
+        squeeze = len(sh) == 2
         if squeeze:
-            B, (M, ak) = 1, A.shape
-        elif A.dim() == 3:
-            B, M, ak = A.shape
+            B, (M, ak) = 1, sh
+        elif len(sh) == 3:
+            B, M, ak = sh
         else:
-            raise ValueError(f"A: expected [M, K] or [B, M, K], got {tuple(A.shape)}")
-        if ak > 1 and A.stride(-1) != 1:
+            raise ValueError(f"A: expected [M, K] or [B, M, K], got {tuple(sh)}")
+        st = A.stride()
+        if ak > 1 and st[-1] != 1:
             A = A.contiguous()
-        lda = A.stride(-2) if M > 1 else 0
-        abs_ = A.stride(0) if B > 1 else 0
+            st = A.stride()
+        if M > 1:
+            lda = st[-2]
+        if B > 1:
+            abs_ = st[0]
     if ak != K:
         raise ValueError(f"A has K = {ak}, W has K = {K}")
     if epilogue not in (EPI_BIAS, EPI_BIAS_GELU_TANH, EPI_BIAS_GATE_RES, EPI_F32_OUT):
@@ -382,8 +388,12 @@ def gemm_mxfp4(A: Union[torch.Tensor, Mxfp4], W: Mxfp4, bias: Optional[torch.Ten
         need = _lib.load().ea_gemm_mxfp4_workspace_bytes(B, M, N, K, not packed)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         qa, sa, x = (A.codes.data_ptr(), A.scales.data_ptr(), None) if packed else (None, None, A.data_ptr())
-        _timed("gemm", lambda: _lib.call("ea_gemm_mxfp4", qa, sa, x, W.codes.data_ptr(), W.scales.data_ptr(), _a(bias), out.data_ptr(), _a(res), _a(gate),
-                                         B, M, N, K, lda, abs_, ldc, cbs, ldres, rbs, gbs, epilogue, _a(ws), need, _stream_on(dev)))
+        args = (qa, sa, x, W.codes.data_ptr(), W.scales.data_ptr(), _a(bias), out.data_ptr(), _a(res), _a(gate), B, M, N, K, lda, abs_, ldc, cbs, ldres, rbs,
+                gbs, epilogue, _a(ws), need, _stream_on(dev))
+        if KernelTimer.active is None:
+            _lib.call("ea_gemm_mxfp4", *args)
+        else:
+            _timed("gemm", lambda: _lib.call("ea_gemm_mxfp4", *args))
     return out
 
 
@@ -705,17 +715,33 @@ def attention_causal_gqa(q: torch.Tensor, k: torch.Tensor, vt: torch.Tensor, seq
     return out
 
 
-def _strided(t: torch.Tensor):
+_I64x11 = ctypes.c_int64 * 11
+
+
+def _strided(t: torch.Tensor, nb: int, nh: int, ns: int):
     """(t, its batch / head / row strides) as ea_attention_text_bf16 reads them: unit inner stride, strides multiples of 8 (those of
     one-element axes do not count), rows less than 2^24 apart, 16-byte aligned -- or a contiguous copy where t is not like that."""
-    sh, (b, h, s, d) = t.shape, t.stride()
-    b, h, s = b if sh[0] > 1 else 0, h if sh[1] > 1 else 0, s if sh[2] > 1 else 0
+    b, h, s, d = t.stride()
+    if nb == 1:
+        b = 0
+    if nh == 1:
+        h = 0
+    if ns == 1:
+        s = 0
     if d != 1 or (b | h | s) & 7 or s >= 1 << 24 or t.data_ptr() & 15:
         t = t.contiguous()
         if t.data_ptr() & 15:
             t = t.clone()
-        return t, (t.stride(0), t.stride(1), t.stride(2))
-    return t, (b, h, s)
+        b, h, s, _ = t.stride()
+    return t, b, h, s
+
+
+def _ints(t: torch.Tensor, name: str, *shape: int) -> int:
+    """Address of an int32 tensor of this shape with unit inner stride."""
+    _chk(t, torch.int32, name)
+    if t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name}: expected {shape} with unit inner stride, got {tuple(t.shape)}, strides {t.stride()}")
+    return t.data_ptr()
 
 
 def attention_text(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, *, causal: bool = False, cap: float = 0.0,
@@ -732,54 +758,67 @@ def attention_text(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: flo
       q_start      int32 [B]: position of the first query (default Sk - Sq: the queries are the last tokens)
     A query that sees no key gives zeros.  One new token against a long cache is split over the GPU.  out must not overlap q, k or v.
     (ea_attention_text_bf16)"""
-    _chk(q, _BF16, "q"); _chk(k, _BF16, "k"); _chk(v, _BF16, "v")
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"q, k, v: expected [B, H, S, D] with k and v alike, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    B, Hq, Sq, D = q.shape
-    Hkv, Sk = k.shape[1], k.shape[2]
-    if k.shape[0] != B or k.shape[3] != D or Hkv < 1 or Hq < 1 or Hq % Hkv:
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not belong together (batch, head_dim, heads a multiple of kv heads)")
+    if not (q.dtype == k.dtype == v.dtype == _BF16):
+        _chk(q, _BF16, "q"); _chk(k, _BF16, "k"); _chk(v, _BF16, "v")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape:
+        raise ValueError(f"q, k, v: expected [B, H, S, D] with k and v alike, got {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}")
+    B, Hq, Sq, D = qs
+    kb, Hkv, Sk, kd = ks
+    if kb != B or kd != D or Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"q {tuple(qs)} and k {tuple(ks)} do not belong together (batch, head_dim, heads a multiple of kv heads)")
     if D not in (64, 128):
         raise ValueError(f"head_dim {D}: 64 and 128 are built")
     if not (0.0 < scale <= 1e30) or not (cap == 0.0 or (1e-30 <= cap <= 1e30 and scale <= 1e30 * cap)):
         raise ValueError(f"scale must be positive and at most 1e30, cap 0 or between 1e-30 and 1e30 (got {scale}, {cap})")
-    reach = 0
+    reach, qd_ld, kd_ld = 0, 0, 0
+    a_bias = a_qd = a_kd = a_prefix = a_valid = a_start = None
     if bias is not None:
         _chk(bias, _F32, "bias")
         if bias.dim() != 2 or bias.shape[0] != Hq or bias.shape[1] % 2 != 1 or not bias.is_contiguous():
             raise ValueError(f"bias: expected contiguous [{Hq}, 2 R + 1], got {tuple(bias.shape)}")
-        reach = bias.shape[1] // 2
+        reach, a_bias = bias.shape[1] // 2, bias.data_ptr()
     if (q_docs is None) != (kv_docs is None):
         raise ValueError("q_docs and kv_docs come together")
     if prefix is not None and not causal:
         raise ValueError("prefix needs causal order")
-    for t, name, shape in ((q_docs, "q_docs", (B, Sq)), (kv_docs, "kv_docs", (B, Sk)), (prefix, "prefix", (B,)), (valid, "valid", (B,)),
-                           (q_start, "q_start", (B,))):
-        if t is not None:
-            _chk(t, torch.int32, name)
-            if t.shape != shape or (t.shape[-1] > 1 and t.stride(-1) != 1):
-                raise ValueError(f"{name}: expected {shape} with unit inner stride, got {tuple(t.shape)}, strides {t.stride()}")
-    with _same_device(q.device, k, v, bias, q_docs, kv_docs, prefix, valid, q_start, out):
+    if q_docs is not None:
+        a_qd, a_kd = _ints(q_docs, "q_docs", B, Sq), _ints(kv_docs, "kv_docs", B, Sk)
+        qd_ld, kd_ld = q_docs.stride(0), kv_docs.stride(0)
+    if prefix is not None:
+        a_prefix = _ints(prefix, "prefix", B)
+    if valid is not None:
+        a_valid = _ints(valid, "valid", B)
+    if q_start is not None:
+        a_start = _ints(q_start, "q_start", B)
+    dev = q.device
+    with _same_device(dev, k, v, bias, q_docs, kv_docs, prefix, valid, q_start, out):
         if out is None:
-            out = torch.empty((B, Sq, Hq * D), dtype=_BF16, device=q.device)
-        _chk(out, _BF16, "out")
-        if out.shape != (B, Sq, Hq * D) or out.stride(2) != 1:
-            raise ValueError(f"out: expected [{B}, {Sq}, {Hq * D}] with unit inner stride, got {tuple(out.shape)}, strides {out.stride()}")
-        if (B > 1 and out.stride(0) < Hq * D) or (Sq > 1 and out.stride(1) < Hq * D):
-            raise ValueError(f"out: rows overlap (strides {out.stride()})")
+            out = torch.empty((B, Sq, Hq * D), dtype=_BF16, device=dev)
+            ob, os_ = Sq * Hq * D, Hq * D
+        else:
+            _chk(out, _BF16, "out")
+            ob, os_, od = out.stride() if out.dim() == 3 else (0, 0, 0)
+            if out.shape != (B, Sq, Hq * D) or od != 1:
+                raise ValueError(f"out: expected [{B}, {Sq}, {Hq * D}] with unit inner stride, got {tuple(out.shape)}, strides {out.stride()}")
+            if (B > 1 and ob < Hq * D) or (Sq > 1 and os_ < Hq * D):
+                raise ValueError(f"out: rows overlap (strides {out.stride()})")
         if B == 0 or Sq == 0:
             return out
         if Sk == 0:
             return out.zero_()
-        (q, sq), (k, sk), (v, sv) = _strided(q), _strided(k), _strided(v)
-        strides = (ctypes.c_int64 * 11)(*sq, *sk, *sv, out.stride(0) if B > 1 else 0, out.stride(1) if Sq > 1 else 0)
-        need = _lib.load().ea_attention_text_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, int(q_docs is not None))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        _timed("attention", lambda: _lib.call("ea_attention_text_bf16", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                              ctypes.addressof(strides), B, Hq, Hkv, Sq, Sk, D, scale, causal, cap, _a(bias), reach, _a(q_docs),
-                                              _a(kv_docs), q_docs.stride(0) if q_docs is not None else 0,
-                                              kv_docs.stride(0) if kv_docs is not None else 0, _a(prefix), _a(valid), _a(q_start), _a(ws), need,
-                                              _stream_on(q.device)))
+        q, qb, qh, qr = _strided(q, B, Hq, Sq)
+        k, kb, kh, kr = _strided(k, B, Hkv, Sk)
+        v, vb, vh, vr = _strided(v, B, Hkv, Sk)
+        strides = _I64x11(qb, qh, qr, kb, kh, kr, vb, vh, vr, ob if B > 1 else 0, os_ if Sq > 1 else 0)
+        need = _lib.load().ea_attention_text_workspace_bytes(B, Hq, Hkv, Sq, Sk, D, a_qd is not None)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides, B, Hq, Hkv, Sq, Sk, D, scale, causal, cap, a_bias, reach, a_qd, a_kd,
+                qd_ld, kd_ld, a_prefix, a_valid, a_start, None if ws is None else ws.data_ptr(), need, _stream_on(dev))
+        if KernelTimer.active is None:
+            _lib.call("ea_attention_text_bf16", *args)
+        else:
+            _timed("attention", lambda: _lib.call("ea_attention_text_bf16", *args))
     return out
 
 
