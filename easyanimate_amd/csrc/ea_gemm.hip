@@ -1457,6 +1457,7 @@ int ea_gemm_mxfp4_w4_launch(const unsigned char* A, const unsigned char* As, int
                             int64_t cbs, int64_t ldres, int64_t rbs, int64_t gbs, int epilogue, hipStream_t st) {
     const int64_t a_rows = (int64_t)batch * M, limit = 0xFFFFFFFFll;
     if (a_rows * kt * 128 >= limit || (int64_t)N * kt * 128 >= limit || as_bytes >= limit || (int64_t)kt * 64 > 0x7fffffff) return EA_ERR_ARG;
+    if (a_rows < 2 || as_bytes < a_rows * kt * 8 + (M % 2 ? MXW4_SCALE_PAD : 0)) return EA_ERR_ARG;      // (what mxw4_scale_offset's pairs reach)
     GemmArgs p;
     p.A = reinterpret_cast<const unsigned short*>(A); p.W = reinterpret_cast<const unsigned short*>(W); p.bias = bias;
     p.C = reinterpret_cast<unsigned short*>(C); p.res = res; p.gate = gate;
