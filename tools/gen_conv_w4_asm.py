@@ -4,8 +4,8 @@ tiles of 16x16x32 = the whole AGPR file), as ONE inline-asm block per tile geome
 
     python tools/gen_conv_w4_asm.py
 
-The same idea as tools/gen_gemm_w4_asm.py (exactly one non-MFMA instruction between two MFMAs, no branch inside the loop body,
-requests beyond the end go through empty buffer resources), on the row-slab data flow of conv3d_cl_row16_k32_kernel:
+The same idea as tools/gen_gemm_w4_asm.py (what is not an MFMA dealt one instruction to a 16-clock MFMA, reads two slots apart, no branch
+inside the loop body, requests beyond the end go through empty buffer resources), on the row-slab data flow of conv3d_cl_row16_k32_kernel:
 
   * a SLAB = one input row segment (TM + 2 voxels x 32 channels, 64-byte LDS rows) for one (dt, dh, channel block); its three
     dw taps are three shifted fragment reads of the same staged rows.  A TILE = (slab, dw) = one k32 step = 64 MFMAs per wave.

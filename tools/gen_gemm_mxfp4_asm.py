@@ -1,5 +1,5 @@
 """Generates easyanimate_amd/csrc/ea_gemm_mxfp4_w4_loop.inc: the hand-placed main loop of gemm256_mxfp4_w4_kernel as ONE inline-asm
-block -- the loop of gen_gemm_w4_asm.py (same tiles in bytes, same fragment buffers, same slots, same hand-overs: see there) on
+block -- the loop of gen_gemm_w4_asm.py (same tiles in bytes, same fragment buffers, same rules for the placement, same hand-overs: see there) on
 v_mfma_scale_f32_16x16x128_f8f6f4, with the scales added:
 
     python tools/gen_gemm_mxfp4_asm.py            (rewrites the .inc)
@@ -45,33 +45,40 @@ def dma_scale():
 def schedule(p):
     """The base schedule plus the scales; p = scale set of this tile (the next tile's pairs go to p ^ 1)."""
     s = g.schedule()
-    assert s[21] == [g.m0_first("w")] and s[22] == []
-    s[20].append(f"s_mov_b32 m0, s{S_MS}")
-    s[21] = [dma_scale()]
-    s[22] = [g.m0_first("w")]
-    s[53].append(f"v_xor_b32 v{V_SW}, 0x1000, v{V_SW}")
-    s[55].append(f"v_xor_b32 v{V_SA}, 0x1000, v{V_SA}")
-    for f, n in enumerate([69, 71, 73, 75, 77, 79, 81, 83, 85, 92, 93, 94, 95, 96, 99, 100]):
+
+    def free(n):
+        while s[n]:
+            n += 1
+        return n
+    # the scale request in front of the W requests, between the barrier that frees their stage and the first of them
+    n = g.REQUEST_W - 1
+    assert s[n][-1] == g.m0_first("w") and g.FREE_W < n
+    s[g.FREE_W].append(f"s_mov_b32 m0, s{S_MS}")
+    s[n].insert(-1, dma_scale())
+    n = g.FREE_A + 1
+    for v in (V_SW, V_SA):
+        n = free(n)
+        s[n].append(f"v_xor_b32 v{v}, 0x1000, v{v}")
+    n = g.READ_W0
+    for f in range(16):
+        n = free(n)
         s[n].append(rd_scale(f, p ^ 1))
-    s[126].append(f"s_add_u32 s{S_KS}, s{S_KS}, s{S_KSTS}")
-    s[127].append(f"s_xor_b32 s{S_MS}, s{S_MS}, 0x1000")
-    # one request more in front of the waits: 8 A(t + 1) + the 11 of this tile in front of slot 68; the 16 in front of slot 105
-    order = [(n, i) for n in range(129) for i in s[n]]
-    vm = [n for n, i in order if i.startswith("buffer_load")]
-    assert len(vm) == 17 and vm[0] == 21
-    s[68] = [f"s_waitcnt vmcnt({8 + sum(n < 68 for n in vm)})", "s_barrier"] + s[68][2:]
-    s[105] = [f"s_waitcnt vmcnt({sum(n < 105 for n in vm)})", "s_barrier"] + s[105][2:]
-    assert "vmcnt(19)" in s[68][0] and "vmcnt(16)" in s[105][0]
-    # no scale register of the set in use is written before its last MFMA
-    for n, i in order:
-        if i.startswith("ds_read_u16"):
-            r = int(i.split()[1].strip("v,"))
-            assert SCALE[p ^ 1] <= r < SCALE[p ^ 1] + 16 and n > 68
+    n = g.REQUEST_A + 7 * g.REQUEST_STEP + 1
+    for ins in (f"s_add_u32 s{S_KS}, s{S_KS}, s{S_KSTS}", f"s_xor_b32 s{S_MS}, s{S_MS}, 0x1000"):
+        n = free(n)
+        s[n].append(ins)
+    s = g.finish(s)
+    # no scale register of the set in use is written before its last MFMA; scale reads end where the fragment reads do
+    for n in s:
+        for i in s[n]:
+            if i.startswith("ds_read_u16"):
+                r = int(i.split()[1].strip("v,"))
+                assert SCALE[p ^ 1] <= r < SCALE[p ^ 1] + 16 and g.LANDED_W < n <= 128 - g.LATENCY
     return s
 
 
 def loop_body():
-    base = g.loop_body(g.schedule(), False, True)
+    base = g.loop_body(g.finish(g.schedule()), False, True)
     body = []
     B = body.append
     # ---- the base prologue up to its first K tile, with the scale resource, addresses, requests and first reads put in

@@ -3,33 +3,40 @@ inline-asm block, plus the accumulator read-out statements.
 
     python tools/gen_gemm_w4_asm.py            (rewrites the .inc; the build hashes it like every source file)
 
-Why generated: the loop is 128 MFMAs per K tile with exactly one other instruction between two MFMAs, on fixed registers
+Why generated: the loop is 128 MFMAs per K tile with the other instructions dealt between them, on fixed registers
 (accumulators a0..a255, fragment double buffer v0..v127) -- placing ~330 lines by hand once per schedule experiment is what
-this script is for.  The SCHEDULE table below is the whole design; everything else is bookkeeping.
+this script is for.
 
 Structure (one wave per SIMD, 128 x 128 wave tile = 8 x 8 MFMA tiles of 16x16x32, K tile = 2 k-steps of 64 MFMAs):
-  slot n = "in front of MFMA n" of the K tile.  k-step 0 (slots 0..63) computes on fragment buffer 0, k-step 1 on buffer 1.
-  W = weight operand, A = activation operand; stage s holds tile t, tile t+1 is landing in stage s^1, tile t+2 is requested
-  into stage s as soon as ALL waves have the corresponding operand of tile t in registers (one barrier per operand):
-     1..15   ds_read W k-step-1 fragments of tile t           -> buffer 1
-     20      lgkmcnt(0) + barrier: W(t) is in registers everywhere -> W region of stage s is free
-     23..59  8 x LDS-DMA W(t+2) -> stage s, interleaved with ds_read A k-step-1 fragments (25..43)
-     51      lgkmcnt(0) + barrier: A(t) is in registers everywhere -> A region of stage s is free
-     62..125 8 x LDS-DMA A(t+2) -> stage s
-     68      vmcnt(18) + barrier: W(t+1) has landed (own pieces by count, the others' by the barrier)
-     70..84  ds_read W k-step-0 fragments of tile t+1          -> buffer 0 (its last reader was MFMA 63)
-     105     vmcnt(15) + barrier: A(t+1) has landed
-     107..121 ds_read A k-step-0 fragments of tile t+1         -> buffer 0
-  No branch inside the tile: the requests of tiles >= nk go through a buffer resource with num_records = 0 (no traffic, the
-  vmcnt bookkeeping stays uniform)."""
+  slot n = "in front of MFMA n" of the K tile; an MFMA takes 16 clocks, so a K tile is 2 048.  k-step 0 (slots 0..63) computes on fragment
+  buffer 0, k-step 1 on buffer 1.  W = weight operand, A = activation operand.  Two stages of both operands are 128 of the 160 KiB of
+  LDS, a third does not fit: stage s holds tile t, tile t + 1 is landing in stage s ^ 1, and tile t + 2 can be requested into stage s
+  only when ALL waves hold an operand of tile t in registers, hence one barrier behind the reads of each operand and one in front.
+
+Everything else is placed by four rules (the constants below):
+  * fragment reads 2 slots apart: the four waves of a CU together read 4 KiB per 32 clocks, the 128 bytes a clock that LDS delivers;
+  * LATENCY slots between a read and the wait for it (LDS answers in about 128 clocks);
+  * the reads of tile t + 1 as late as that allows, so that its requests have the longest time in flight: the activation reads end
+    LATENCY slots in front of the next tile, the weight reads begin where buffer 0 is free (its last reader is MFMA 63);
+  * the 16 LDS-DMA requests evenly over what is left behind the first release, REQUEST_STEP slots apart: L2 feeds a CU's LDS no faster
+    than about 32 bytes a clock, which is the 64 KiB of a K tile in its 2 048 clocks, and a burst of them holds the wave at issue.
+  No branch inside the tile: the requests of tiles >= nk go through a buffer resource with num_records = 0 (no traffic, the vmcnt
+  bookkeeping stays uniform).  The waits' counts are computed from the table (finish())."""
 import os
 
-# schedule experiments (the committed .inc is generated with the defaults): EA_W4A_TOP=prog -> progressive lgkmcnt waits in front of
-# the first eight MFMAs of a tile instead of one full drain; EA_W4A_BAR1=<slot> -> the "W(t) consumed" barrier (default 20)
-TOP_PROG = os.environ.get("EA_W4A_TOP", "drain") == "prog"
-BAR1 = int(os.environ.get("EA_W4A_BAR1", "20"))
-
 OUT = os.environ.get("EA_GEN_OUT") or os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "easyanimate_amd", "csrc", "ea_gemm_w4_loop.inc")     # EA_GEN_OUT: write somewhere else (tests/test_w4a_isa_cpu.py compares with the committed file)
+
+READ_STEP, LATENCY, REQUEST_STEP = 2, 8, 6
+READ_W1 = 1                                           # first read of W's k-step-1 fragments
+READ_A1 = READ_W1 + 8 * READ_STEP                     # .. of A's, right behind
+FREE_W = READ_A1 + LATENCY - 1                        # W(t) is in registers everywhere
+FREE_A = READ_A1 + 8 * READ_STEP + LATENCY - 1
+REQUEST_W = FREE_W + 2
+REQUEST_A = REQUEST_W + 8 * REQUEST_STEP
+READ_A0 = 128 - LATENCY - 8 * READ_STEP + 1           # k-step-0 fragments of tile t + 1
+LANDED_A = READ_A0 - 1
+LANDED_W = 66
+READ_W0 = LANDED_W + 1
 
 # fixed registers
 FW = [0, 64]      # first VGPR of W fragment buffer b (8 fragments x 4 registers)
@@ -81,66 +88,78 @@ M0_NEXT = "s_add_u32 m0, m0, 0x400"
 
 
 def schedule():
-    """slot -> instructions placed in front of MFMA `slot` of the K tile."""
+    """slot -> instructions placed in front of MFMA `slot` of the K tile; "<..>" are the waits, filled in by finish()."""
     s = {n: [] for n in range(129)}
-    for x in range(8):                                   # W k-step 1 of tile t
-        s[1 + 2 * x].append(rd("w", 1, x, "wk1"))
-    s[17].append(f"v_xor_b32 v{ADDR['wk1']}, 0x8000, v{ADDR['wk1']}")     # -> the other stage, for the next tile
-    s[BAR1] += ["s_waitcnt lgkmcnt(0)", "s_barrier"]
-    s[BAR1 + 1].append(m0_first("w"))
-    w_slots = [BAR1 + 3, BAR1 + 6, BAR1 + 9, BAR1 + 12, BAR1 + 15, 53, 56, 59]
-    for x, n in enumerate(w_slots):                       # W(t+2)
-        s[n].append(dma("w", x))
-        if x < 7:
-            s[n + 1].append(M0_NEXT)
-    a1_slots = [25, 28, 31, 34, 37, 39, 41, 43]
-    for x, n in enumerate(a1_slots):                      # A k-step 1 of tile t
-        s[n].append(rd("a", 1, x, "ak1"))
-    s[45].append(f"v_xor_b32 v{ADDR['ak1']}, 0x8000, v{ADDR['ak1']}")
-    s[47].append(f"v_xor_b32 v{ADDR['wk0']}, 0x8000, v{ADDR['wk0']}")
-    s[49].append(f"v_xor_b32 v{ADDR['ak0']}, 0x8000, v{ADDR['ak0']}")
-    s[51] += ["s_waitcnt lgkmcnt(0)", "s_barrier"]
-    s[60].append(m0_first("a"))
-    a_slots = [62, 65, 86, 88, 90, 97, 101, 125]
-    for x, n in enumerate(a_slots):                       # A(t+2)
-        s[n].append(dma("a", x))
-        if x < 7:
-            s[n + 1].append(M0_NEXT)
-    s[68] += ["s_waitcnt vmcnt(18)", "s_barrier"]
-    for x in range(8):                                    # W k-step 0 of tile t+1
-        s[70 + 2 * x].append(rd("w", 0, x, "wk0"))
-    s[105] += ["s_waitcnt vmcnt(15)", "s_barrier"]
-    for x in range(8):                                    # A k-step 0 of tile t+1
-        s[107 + 2 * x].append(rd("a", 0, x, "ak0"))
+
+    def free(n):                                          # the next slot from n on with nothing in it
+        while s[n]:
+            n += 1
+        return n
+    for x in range(8):
+        s[READ_W1 + READ_STEP * x].append(rd("w", 1, x, "wk1"))
+        s[READ_A1 + READ_STEP * x].append(rd("a", 1, x, "ak1"))
+        s[READ_W0 + READ_STEP * x].append(rd("w", 0, x, "wk0"))
+        s[READ_A0 + READ_STEP * x].append(rd("a", 0, x, "ak0"))
+    s[FREE_W] += ["<w free>", "s_barrier"]
+    s[FREE_A] += ["<a free>", "s_barrier"]
+    s[LANDED_W] += ["<w landed>", "s_barrier"]
+    s[LANDED_A] += ["<a landed>", "s_barrier"]
+    for oper, first in (("w", REQUEST_W), ("a", REQUEST_A)):
+        for x in range(8):
+            s[first + REQUEST_STEP * x].append(dma(oper, x))
+    for oper, first in (("w", REQUEST_W), ("a", REQUEST_A)):      # m0 one slot or more in front of its request, behind the one before
+        s[first - 1].append(m0_first(oper))
+        for x in range(7):
+            n = free(first + REQUEST_STEP * x + 1)
+            assert n < first + REQUEST_STEP * (x + 1)
+            s[n].append(M0_NEXT)
+    # the addresses go to the other stage: k-step 1 behind its last read, k-step 0 between two tiles' reads
+    s[free(READ_A1)].append(f"v_xor_b32 v{V_WK1}, 0x8000, v{V_WK1}")
+    s[free(READ_A1 + 8 * READ_STEP)].append(f"v_xor_b32 v{V_AK1}, 0x8000, v{V_AK1}")
+    s[free(FREE_A + 1)].append(f"v_xor_b32 v{V_WK0}, 0x8000, v{V_WK0}")
+    s[free(FREE_A + 1)].append(f"v_xor_b32 v{V_AK0}, 0x8000, v{V_AK0}")
     # scalar bookkeeping of the next tile, behind the last request
-    s[126] += [f"s_add_u32 s{S_KA}, s{S_KA}, s{S_KSTA}", f"s_add_u32 s{S_KW}, s{S_KW}, s{S_KSTW}"]
-    s[127] += [f"s_xor_b32 s{S_MW}, s{S_MW}, 0x8000", f"s_xor_b32 s{S_MA}, s{S_MA}, 0x8000", f"s_sub_u32 s{S_LEFT}, s{S_LEFT}, 1"]
+    n = REQUEST_A + 7 * REQUEST_STEP + 1
+    for ins in (f"s_add_u32 s{S_KA}, s{S_KA}, s{S_KSTA}", f"s_add_u32 s{S_KW}, s{S_KW}, s{S_KSTW}", f"s_xor_b32 s{S_MW}, s{S_MW}, 0x8000",
+                f"s_xor_b32 s{S_MA}, s{S_MA}, 0x8000", f"s_sub_u32 s{S_LEFT}, s{S_LEFT}, 1"):
+        n = free(n)
+        s[n].append(ins)
     return s
 
 
-def check(s):
-    """The counts the waits rely on."""
-    order = []
-    for n in range(129):
-        for ins in s[n]:
-            order.append((n, ins))
-    dmas = [(n, i) for n, i in order if i.startswith("buffer_load")]
-    assert len(dmas) == 16 and all("woff" in i for _, i in dmas[:8]) and all("aoff" in i for _, i in dmas[8:])
-    before68 = sum(1 for n, _ in dmas if n < 68)
-    before105 = sum(1 for n, _ in dmas if n < 105)
-    assert before68 == 10 and before105 == 15, (before68, before105)     # vmcnt(8 + 10) / vmcnt(15)
-    reads = [(n, i) for n, i in order if i.startswith("ds_read")]
-    assert len(reads) == 32
-    # a register written by a read must not be read by an MFMA that is still to come in the same role
-    for n, i in reads:
-        b = 1 if (f"v{V_WK1}" in i.split("],")[1] or f"v{V_AK1}" in i.split("],")[1]) else 0
-        first_use, last_use_prev = (64, 128) if b == 1 else (128, 64)   # buffer 0 is next used by the NEXT tile's MFMA 0
-        if b == 1:
-            assert n < 64
-        else:
-            assert n >= 64
-    # m0 is written at least one instruction before each DMA and never between the DMA and its own m0
-    return True
+def finish(s):
+    """The waits' counts from the table, and what the loop relies on."""
+    order = [(n, i) for n in range(129) for i in s[n]]
+    at = {i: k for k, (_, i) in enumerate(order) if i.startswith("<")}
+    reads = [(k, n, i) for k, (n, i) in enumerate(order) if i.startswith("ds_read_b128")]
+    dmas = [(k, n, i) for k, (n, i) in enumerate(order) if i.startswith("buffer_load")]
+
+    def of(addr):
+        return [(k, n) for k, n, i in reads if f"v{ADDR[addr]}" in i.split("],")[1]]
+    lds = [k for k, (_, i) in enumerate(order) if i.startswith("ds_read")]
+    w_dma, a_dma = [k for k, _, i in dmas if "%[woff" in i], [k for k, _, i in dmas if "%[aoff" in i]
+    assert len(reads) == 32 and len(w_dma) == 8 and len(a_dma) == 8 and max(w_dma) < min(a_dma)
+    for addr in ADDR:
+        assert len(of(addr)) == 8
+    # requests of tile t + 2 behind the barrier that frees their operand's stage; LDS reads answer in order
+    assert max(k for k, _ in of("wk1")) < at["<w free>"] < min(k for k, _, i in dmas if "%[aoff" not in i)
+    assert max(k for k, _ in of("ak1")) < at["<a free>"] < min(a_dma) and order[at["<a free>"]][0] <= 64 - LATENCY
+    w_left = sum(max(k for k, _ in of("wk1")) < k < at["<w free>"] for k in lds)
+    assert w_left <= 15
+    # reads of tile t + 1 behind the barrier that says it has landed, and not before buffer 0's last reader
+    assert min(k for k, _ in of("wk0")) > at["<w landed>"] and min(k for k, _ in of("ak0")) > at["<a landed>"] > at["<w landed>"]
+    assert min(n for _, n in of("wk0") + of("ak0")) >= 64 and max(n for _, n in of("wk1") + of("ak1")) < 64
+    before = lambda w: sum(k < at[w] for k, _, _ in dmas)
+    fill = {"<w free>": f"s_waitcnt lgkmcnt({w_left})", "<a free>": "s_waitcnt lgkmcnt(0)",
+            # requests in order: W(t + 1), A(t + 1) of the tile before, then this tile's
+            "<w landed>": f"s_waitcnt vmcnt({8 + before('<w landed>')})", "<a landed>": f"s_waitcnt vmcnt({before('<a landed>')})"}
+    # m0: written at least one instruction in front of each request, and once between two
+    prev = 0
+    for k, _, _ in dmas:
+        m0 = [j for j in range(prev, k) if " m0," in order[j][1]]
+        assert len(m0) == 1 and (order[m0[0]][0] < order[k][0] or m0[0] < k - 1), (order[k], m0)
+        prev = k
+    return {n: [fill.get(i, i) for i in s[n]] for n in s}
 
 
 def loop_body(s, swap, bias_gate=False):
@@ -222,13 +241,8 @@ def loop_body(s, swap, bias_gate=False):
         B(f"s_cmp_gt_u32 s{S_LEFT}, 2")                # tile t + 2 exists?
         B(f"s_cselect_b32 s{S_RA + 2}, s{S_NRA}, 0")
         B(f"s_cselect_b32 s{S_RW + 2}, s{S_NRW}, 0")
-        if not TOP_PROG:
-            B("s_waitcnt lgkmcnt(0)")                  # buffer 0 = k-step 0 of this tile
+        B("s_waitcnt lgkmcnt(0)")                      # buffer 0 = k-step 0 of this tile
         for n in range(128):
-            if TOP_PROG and n < 8:
-                # MFMA n needs activation fragment n (the eight A reads are the youngest of the previous tile, in order); W k-step-1
-                # reads issued at the odd slots before this point are younger still
-                B(f"s_waitcnt lgkmcnt({7 - n + n // 2})")
             for ins in s[n]:
                 if first and nbg and ins.startswith("s_waitcnt vmcnt("):
                     ins = f"s_waitcnt vmcnt({int(ins[len('s_waitcnt vmcnt('):-1]) + nbg})"
@@ -254,8 +268,7 @@ def loop_body(s, swap, bias_gate=False):
 
 
 def emit():
-    s = schedule()
-    check(s)
+    s = finish(schedule())
     L = []
     A = L.append
     A("// GENERATED by tools/gen_gemm_w4_asm.py -- do not edit; see that file for the schedule.")
