@@ -50,6 +50,11 @@ def _find_text_model(hf_model):
     raise TypeError(f"{type(hf_model).__name__}: no decoder stack (layers / embed_tokens / norm) found")
 
 
+def _check_weights(weights: str) -> None:
+    if weights not in ("bf16", "mxfp4"):
+        raise ValueError(f"weights must be 'bf16' or 'mxfp4', not {weights!r}")
+
+
 class Qwen2VLTextEncoderHIP(nn.Module):
     def __init__(self, hf_model, padded_positions: str = "arange", weights: str = "bf16"):
         """padded_positions: the rotary position of the right-PADDED slots (real tokens are 0 .. n-1 either way; the DiT consumes
@@ -59,8 +64,7 @@ class Qwen2VLTextEncoderHIP(nn.Module):
         super().__init__()
         if padded_positions not in ("arange", "cumsum_fill1"):
             raise ValueError(f"padded_positions must be 'arange' or 'cumsum_fill1', not {padded_positions!r}")
-        if weights not in ("bf16", "mxfp4"):
-            raise ValueError(f"weights must be 'bf16' or 'mxfp4', not {weights!r}")
+        _check_weights(weights)
         self.padded_positions = padded_positions
         self.weights = weights
         self.hf = hf_model                                 # (registered: .to() / offload hooks reach the shared parameters)
@@ -188,9 +192,14 @@ class Qwen2VLTextEncoderHIP(nn.Module):
 
 
 def use_hip_text_encoder(pipeline, index: int = 0, weights: str = "bf16"):
-    """Swap the transformers model in a pipeline's text_encoder slot for its device-library forward (weights shared)."""
+    """Swap the transformers model in a pipeline's text_encoder slot for its device-library forward (weights shared).  A slot that holds
+    one already is left as it is, or, where its `weights` differ from what is asked for, gets one with those around the same model."""
+    _check_weights(weights)
     name = "text_encoder" if index == 0 else "text_encoder_2"
     enc = getattr(pipeline, name)
-    if enc is not None and not isinstance(enc, Qwen2VLTextEncoderHIP):
+    if isinstance(enc, Qwen2VLTextEncoderHIP):
+        if enc.weights != weights:
+            setattr(pipeline, name, Qwen2VLTextEncoderHIP(enc.hf, enc.padded_positions, weights).train(enc.training))
+    elif enc is not None:
         setattr(pipeline, name, Qwen2VLTextEncoderHIP(enc, weights=weights))
     return getattr(pipeline, name)
