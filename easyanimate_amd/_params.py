@@ -9,7 +9,7 @@ from typing import Callable, Dict, Tuple
 
 import torch
 
-_cache: Dict[Tuple[int, str], Tuple[tuple, torch.Tensor]] = {}
+_cache: Dict[Tuple[int, str], tuple] = {}      # (signature, derived copy, _Made or None)
 _finalized: set = set()      # (id(parameter), tag) keys that already carry a weakref.finalize
 
 
@@ -17,15 +17,53 @@ def _key(p: torch.Tensor):
     return (p.data_ptr(), p._version, p.device, p.dtype, tuple(p.shape))
 
 
+def _raw_stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _capturing(dev: torch.device) -> bool:
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
+class _Made:
+    """Where a derived copy was made: the stream, an event behind its kernels, and the streams that already stand behind that."""
+    __slots__ = ("event", "streams")
+
+    def __init__(self, dev: torch.device):
+        self.event = torch.cuda.Event()
+        self.event.record(torch.cuda.current_stream(dev))
+        self.streams = {_raw_stream(dev)}
+
+    def join(self, dev: torch.device, val) -> None:
+        """Before the current stream of `dev` reads the copy: it waits for it, and the copy's memory is not used again, once it is
+        dropped, before that stream is through with it.  (Under capture nothing is to be waited for: the device was idle when it began,
+        and an event from outside may not enter a graph.)"""
+        raw = _raw_stream(dev)
+        if raw in self.streams or _capturing(dev):
+            return
+        stream = torch.cuda.current_stream(dev)
+        stream.wait_event(self.event)
+        for t in (val,) if isinstance(val, torch.Tensor) else (val.codes, val.scales):
+            t.record_stream(stream)
+        self.streams.add(raw)
+
+
 def derived(p: torch.Tensor, tag: str, fn: Callable[[torch.Tensor], torch.Tensor]) -> torch.Tensor:
+    """fn(p), kept until p changes; usable on any stream.  Made under graph capture it belongs to the graph (its memory is filled by
+    replays) and is not kept."""
     k = (id(p), tag)
     ent = _cache.get(k)
     sig = _key(p)
     if ent is not None and ent[0] == sig:
+        if ent[2] is not None:
+            ent[2].join(p.device, ent[1])
         return ent[1]
     with torch.no_grad():
         val = fn(p.detach())
-    _cache[k] = (sig, val)
+    if p.is_cuda and _capturing(p.device):
+        return val
+    _cache[k] = (sig, val, _Made(p.device) if p.is_cuda else None)
     if k not in _finalized:      # ONE finalizer per (parameter, tag) for the parameter's lifetime: every pipeline call clears the
         try:                     # cache (invalidate_weight_cache) and recomputes -- it must not also add a finalizer each time
             weakref.finalize(p, _drop, k)

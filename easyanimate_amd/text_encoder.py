@@ -29,7 +29,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from ._params import f32, gemm_weight, mxfp4_weight
+from ._params import derived, f32, gemm_weight, mxfp4_weight
 
 
 def _find_text_model(hf_model):
@@ -86,7 +86,6 @@ class Qwen2VLTextEncoderHIP(nn.Module):
         if getattr(cfg, "hidden_act", "silu") != "silu":
             raise NotImplementedError(f"Qwen2VLTextEncoderHIP: hidden_act {cfg.hidden_act!r}")
         self._text = [text]                                # (a list: not registered a second time)
-        self._ones = {}
 
     # ---- what the pipelines read -------------------------------------------------------------
     @property
@@ -101,15 +100,12 @@ class Qwen2VLTextEncoderHIP(nn.Module):
     def config(self):
         return self.hf.config
 
-    def _gate_ones(self, n: int, device) -> torch.Tensor:
-        key = (n, str(device))
-        if key not in self._ones:
-            self._ones[key] = torch.ones(n, dtype=torch.float32, device=device)
-        return self._ones[key]
+    def _gate_ones(self) -> torch.Tensor:
+        return derived(self._text[0].norm.weight, "ones", lambda t: torch.ones(self.hidden, dtype=torch.float32, device=t.device))
 
     def _layer_mxfp4(self, layer, h, B, S, cos, sin, valid):
         att, mlp, D, Hq, Hkv = layer.self_attn, layer.mlp, self.head_dim, self.q_heads, self.kv_heads
-        ones = self._gate_ones(self.hidden, h.device)
+        ones = self._gate_ones()
         fb = lambda lin: f32(lin.bias) if lin.bias is not None else None
         lin = lambda a, l: ops.gemm_mxfp4(a, mxfp4_weight(l.weight), fb(l))
         add = lambda a, l, res: ops.gemm_mxfp4(a, mxfp4_weight(l.weight), fb(l), ops.EPI_BIAS_GATE_RES, res=res, gate=ones)
@@ -178,12 +174,12 @@ class Qwen2VLTextEncoderHIP(nn.Module):
             vt[..., :S] = v.view(B, S, Hkv, D).permute(0, 2, 3, 1)            # V^T (columns >= S stay zero)
             a = ops.attention_causal_gqa(qh, kh, vt, S, D ** -0.5, valid)
             ob = f32(att.o_proj.bias) if att.o_proj.bias is not None else None
-            h = ops.gemm(a.view(B * S, Hq * D), gemm_weight(att.o_proj.weight), ob, ops.EPI_BIAS_GATE_RES, res=h, gate=self._gate_ones(d, dev))
+            h = ops.gemm(a.view(B * S, Hq * D), gemm_weight(att.o_proj.weight), ob, ops.EPI_BIAS_GATE_RES, res=h, gate=self._gate_ones())
             n2 = ops.rmsnorm(h, f32(layer.post_attention_layernorm.weight), self.eps)
             g = ops.gemm(n2, gemm_weight(mlp.gate_proj.weight), None)
             u = ops.gemm(n2, gemm_weight(mlp.up_proj.weight), None)
             act = ops.silu_mul(g, u)
-            h = ops.gemm(act, gemm_weight(mlp.down_proj.weight), None, ops.EPI_BIAS_GATE_RES, res=h, gate=self._gate_ones(d, dev))
+            h = ops.gemm(act, gemm_weight(mlp.down_proj.weight), None, ops.EPI_BIAS_GATE_RES, res=h, gate=self._gate_ones())
             hidden_states.append(h.view(B, S, d))
         last = ops.rmsnorm(h, f32(text.norm.weight), self.eps).view(B, S, d)
         # transformers: hidden_states = (embeddings, layer 1 .. layer L-1 outputs, NORMED layer L output)

@@ -1,0 +1,59 @@
+"""The 4-bit text encoder's kept weights (weights_frozen): used from several streams, dropped while another stream still reads, and from
+captured graphs."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(__file__))
+from test_text_encoder_gpu import CASES, _prompt_batch, _qwen
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture()
+def enc():
+    from easyanimate_amd.text_encoder import Qwen2VLTextEncoderHIP
+    c = CASES["hd64"]
+    e = Qwen2VLTextEncoderHIP(_qwen(c["hidden"], c["heads"], c["kv_heads"], c["inter"], c["layers"]).to(torch.bfloat16).to(DEV), weights="mxfp4")
+    ids, _ = _prompt_batch(c["B"], c["S"], 512, c["lens"])
+    ids = ids.to(DEV)
+    return e, lambda: e(input_ids=ids, output_hidden_states=True).hidden_states[-1]
+
+
+def test_second_stream_waits_for_the_first_ones_weights(enc):
+    from easyanimate_amd._params import weights_frozen
+    e, run = enc
+    want = run()
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        with weights_frozen():
+            with torch.cuda.stream(a):
+                torch.cuda._sleep(20_000_000)              # the weights are laid out behind this
+                one = run()
+            with torch.cuda.stream(b):
+                two = run()
+        torch.cuda.synchronize()
+        assert torch.equal(one, want) and torch.equal(two, want)
+
+
+def test_first_use_on_two_streams_at_once(enc):
+    """Nothing of the encoder's is made before: the gate vector and the weights of the first stream are the second one's too."""
+    from easyanimate_amd import _params
+    e, run = enc
+    want = run()
+    for _ in range(3):
+        torch.cuda.synchronize()
+        _params.invalidate_weight_cache()
+        a, b = torch.cuda.Stream(), torch.cuda.Stream()
+        with _params.weights_frozen():
+            with torch.cuda.stream(a):
+                torch.cuda._sleep(20_000_000)
+                one = run()
+            with torch.cuda.stream(b):
+                two = run()
+        torch.cuda.synchronize()
+        assert torch.equal(one, want) and torch.equal(two, want)
