@@ -104,14 +104,14 @@ class weights_frozen:
 
     def __enter__(self):
         global _frozen
-        if _frozen == 0:
-            drop_tag("mxfp4")        # (what an earlier region laid out may be older than a `.data` write since)
         _frozen += 1
         return self
 
     def __exit__(self, *exc):
         global _frozen
         _frozen -= 1
+        if _frozen == 0:
+            drop_tag("mxfp4")        # kept for the region only: memory, and a later `.data` write would not be seen
         return False
 
 

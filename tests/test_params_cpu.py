@@ -84,3 +84,33 @@ def test_capture_waits_for_nothing(gpu):
     assert _params.derived(w, "f32", gpu.make) is one and len(gpu.log) == n
     gpu.capture = False
     assert _params.derived(w, "f32", gpu.make) is one and gpu.log[n] == ("wait", 2)
+
+
+@pytest.fixture()
+def stored(gpu, monkeypatch):
+    from easyanimate_amd import ops
+    monkeypatch.setattr(ops, "mxfp4_quantize", gpu.make)
+    return lambda: [k for k in _params._cache if k[1] == "mxfp4"]
+
+
+def test_4_bit_copies_live_in_their_region(gpu, stored):
+    w = Weight()
+    assert _params.mxfp4_weight(w) is not _params.mxfp4_weight(w) and not stored()
+    with _params.weights_frozen():
+        one = _params.mxfp4_weight(w)
+        with _params.weights_frozen():
+            assert _params.mxfp4_weight(w) is one
+        assert _params.mxfp4_weight(w) is one and len(stored()) == 1        # the inner region's end drops nothing
+    assert not stored()
+    with pytest.raises(KeyError):
+        with _params.weights_frozen():
+            _params.mxfp4_weight(w)
+            raise KeyError
+    assert not stored() and not _params.frozen()
+
+
+def test_other_copies_outlive_the_region(gpu, stored):
+    w = Weight()
+    with _params.weights_frozen():
+        one = _params.derived(w, "kblock", gpu.make)
+    assert _params.derived(w, "kblock", gpu.make) is one
