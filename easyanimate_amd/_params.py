@@ -157,10 +157,11 @@ def bf16_weight(p, k_pad: int | None = None):
 def mxfp4_weight(p):
     """The microscaled 4-bit storage (ops.Mxfp4, 17 / 32 byte per weight) of a Linear weight [N, K].  Kept inside a weights_frozen()
     region only: outside of it laid out anew on every use, so that a write through `.data` is seen too (like kblocked_weight; 2.5 bytes
-    of traffic per weight, 25 us for 3584 x 18944)."""
+    of traffic per weight, 25 us for 3584 x 18944).  So it is under graph capture, in a region too: the graph outlives the region, and
+    its replays lay out the weights as they are then, in the graph's own memory."""
     from . import ops
     make = lambda t: ops.mxfp4_quantize(t.to(torch.bfloat16))
-    if not frozen():
+    if not frozen() or (p.is_cuda and _capturing(p.device)):
         with torch.no_grad():
             return make(p.detach())
     return derived(p, "mxfp4", make)

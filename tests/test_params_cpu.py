@@ -114,3 +114,15 @@ def test_other_copies_outlive_the_region(gpu, stored):
     with _params.weights_frozen():
         one = _params.derived(w, "kblock", gpu.make)
     assert _params.derived(w, "kblock", gpu.make) is one
+
+
+def test_4_bit_copies_of_a_graph_are_its_own(gpu, stored):
+    """A kept copy is dropped with its region, a graph is not."""
+    w = Weight()
+    with _params.weights_frozen():
+        one = _params.mxfp4_weight(w)
+        gpu.capture = True
+        two = _params.mxfp4_weight(w)
+        assert two is not one and _params.mxfp4_weight(w) is not two
+        gpu.capture = False
+        assert _params.mxfp4_weight(w) is one

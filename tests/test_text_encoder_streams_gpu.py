@@ -57,3 +57,46 @@ def test_first_use_on_two_streams_at_once(enc):
                 two = run()
         torch.cuda.synchronize()
         assert torch.equal(one, want) and torch.equal(two, want)
+
+
+def test_a_graph_outlives_its_region(enc):
+    """Captured inside a frozen region after a run that kept the weights; replayed behind the region, with other work and writes between."""
+    from easyanimate_amd import _params
+    e, run = enc
+    first = run()
+    with _params.weights_frozen():
+        assert torch.equal(run(), first)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        assert torch.equal(run(), first)
+    weight = e._text[0].layers[0].mlp.up_proj.weight
+    want = first
+    for i in range(4):
+        torch.full((1 << 22,), 0x55, dtype=torch.uint8, device=DEV)         # (what the region held is used for something else)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        assert torch.equal(run(), want), i
+        if i % 2 == 0:
+            weight.data.mul_(-1.0)                                          # a replay sees it as a run does
+            want = run()
+            assert not torch.equal(want, out)
+
+
+def test_captured_without_a_run_before(enc):
+    """The first thing that a fresh encoder does is a capture: what it lays out belongs to the graph, eager calls make their own."""
+    from easyanimate_amd import _params
+    e, run = enc
+    want = run()
+    torch.cuda.synchronize()
+    _params.invalidate_weight_cache()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    assert torch.equal(run(), want)                                         # before any replay
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want) and torch.equal(run(), want)
