@@ -22,8 +22,13 @@ def _raw_stream(dev: torch.device) -> int:
 
 
 def _capturing(dev: torch.device) -> bool:
+    if torch._C._cuda_getDevice() == dev.index:
+        return torch._C._cuda_isCurrentStreamCapturing()
     with torch.cuda.device(dev):
-        return torch.cuda.is_current_stream_capturing()
+        return torch._C._cuda_isCurrentStreamCapturing()
+
+
+_of_graphs: Dict[int, object] = {}      # copies that a captured graph reads: replays may come after the cache has let go of them
 
 
 class _Made:
@@ -37,10 +42,9 @@ class _Made:
 
     def join(self, dev: torch.device, val) -> None:
         """Before the current stream of `dev` reads the copy: it waits for it, and the copy's memory is not used again, once it is
-        dropped, before that stream is through with it.  (Under capture nothing is to be waited for: the device was idle when it began,
-        and an event from outside may not enter a graph.)"""
+        dropped, before that stream is through with it."""
         raw = _raw_stream(dev)
-        if raw in self.streams or _capturing(dev):
+        if raw in self.streams:
             return
         stream = torch.cuda.current_stream(dev)
         stream.wait_event(self.event)
@@ -51,13 +55,17 @@ class _Made:
 
 def derived(p: torch.Tensor, tag: str, fn: Callable[[torch.Tensor], torch.Tensor]) -> torch.Tensor:
     """fn(p), kept until p changes; usable on any stream.  Made under graph capture it belongs to the graph (its memory is filled by
-    replays) and is not kept."""
+    replays) and is not kept; one that is there already when a graph is captured stays for good (nothing is to be waited for there: the
+    device was idle when the capture began, and an event from outside may not enter a graph)."""
     k = (id(p), tag)
     ent = _cache.get(k)
     sig = _key(p)
     if ent is not None and ent[0] == sig:
         if ent[2] is not None:
-            ent[2].join(p.device, ent[1])
+            if _capturing(p.device):
+                _of_graphs[id(ent[1])] = ent[1]
+            else:
+                ent[2].join(p.device, ent[1])
         return ent[1]
     with torch.no_grad():
         val = fn(p.detach())

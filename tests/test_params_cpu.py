@@ -41,6 +41,7 @@ class Gpu:
         monkeypatch.setattr(torch.cuda, "Event", Event)
         monkeypatch.setattr(torch.cuda, "current_stream", stream)
         monkeypatch.setattr(_params, "_cache", {})
+        monkeypatch.setattr(_params, "_of_graphs", {})
 
     def make(self, _):
         part = lambda n: types.SimpleNamespace(record_stream=lambda s: self.log.append((n, s.id)))
@@ -126,3 +127,15 @@ def test_4_bit_copies_of_a_graph_are_its_own(gpu, stored):
         assert two is not one and _params.mxfp4_weight(w) is not two
         gpu.capture = False
         assert _params.mxfp4_weight(w) is one
+
+
+def test_what_a_graph_reads_outlives_the_cache(gpu):
+    w = Weight()
+    one = _params.derived(w, "f32", gpu.make)
+    gpu.capture = True
+    for _ in range(2):
+        assert _params.derived(w, "f32", gpu.make) is one
+    gpu.capture = False
+    _params.invalidate_weight_cache()
+    assert list(_params._of_graphs.values()) == [one]
+    assert _params.derived(w, "f32", gpu.make) is not one                   # eager calls make theirs anew

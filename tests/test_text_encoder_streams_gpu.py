@@ -100,3 +100,21 @@ def test_captured_without_a_run_before(enc):
         out.zero_()
         graph.replay()
         assert torch.equal(out, want) and torch.equal(run(), want)
+
+
+def test_a_graph_outlives_the_cache(enc):
+    """The fp32 biases and gains that a graph reads stay when the cache is cleared (every pipeline call does that)."""
+    from easyanimate_amd import _params
+    e, run = enc
+    want = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for _ in range(3):
+        _params.invalidate_weight_cache()
+        junk = [torch.full((n,), 7.0, device=DEV) for n in (64, 128, 256, 512, 1024) for _ in range(20)]
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(run(), want)
+        del junk
