@@ -9,14 +9,15 @@
 //
 //   gemm_mxfp4_skinny   few rows: 16 weight rows per workgroup, the K tiles dealt to its eight waves, operands straight from memory;
 //                       for M <= 16 the activations may still be bf16 (quantised on the way, same codes as ea_mxfp4_quantize_bf16)
-//   gemm_mxfp4_tile     256 x 128 .. 64 x 64 tiles through LDS, the small ones by two groups of waves, optionally K-split over workgroups (fp32 partial tiles in the caller's workspace,
-//                       joined in a fixed order by gemm_mxfp4_join)
+//   gemm_mxfp4_tile     256 x 128 .. 64 x 64 tiles through LDS, the small ones by two groups of waves, optionally K-split over workgroups
+//                       (fp32 partial tiles in the caller's workspace, joined in a fixed order by gemm_mxfp4_join)
 //   gemm256_mxfp4_w4    256 x 256 tiles with a hand-placed main loop (ea_gemm_mxfp4_w4.inc)
 //
 // What bounds it: the weight bytes for few rows (one token x 3584 x 3584: 5.3 us, x 18944 x 3584: 10), the LDS fill of a CU for tiles up to
 // 128 x 128 (24 - 33 KB per K tile at 130 - 150 GB/s; 512 x 3584 x 18944 in 33 us = 2.1 PFLOP/s with its weights from memory), the matrix
 // pipe at the clock that the power budget leaves for the largest (8192^3 in 219 us = 5.0 PFLOP/s; ea_gemm_bf16 691 us).
 #include "ea_common.h"
+#include "ea_mxfp4_rows.h"
 
 // ea_mxfp4.hip
 int ea_mxfp4_quantize_launch(const unsigned short* x, unsigned char* codes, unsigned char* scales, int64_t rows, int K, int64_t ld, int64_t per,
@@ -433,6 +434,14 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_join_kernel(MxArgs p) {
     mx_store4<EPI>(p, b, m, n0, v, mx_bias(p, n0), mx_gate<EPI>(p, b, n0), mx_res<EPI>(p, b, m, n0));
 }
 
+// a K tile's scales of a row are 8 bytes: stored scales, copied to where the 256 x 256 kernel may read behind the last row
+__global__ __launch_bounds__(256) void copy_scales_kernel(const uint64_t* __restrict__ from, uint64_t* __restrict__ to, int64_t words) {
+    const int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e * 256 < words) to[i + e * 256] = from[i + e * 256];
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 struct MxPlan {
     int cfg, splits;                      // -1 = skinny, else the index of its tile in MX_TILES
@@ -462,7 +471,7 @@ MxPlan mx_plan(int batch, int M, int N, int K, bool from_bf16, bool vec) {
     const int64_t kt = ((int64_t)K + 255) / 256;
     if (from_bf16 && !(M <= 16 && vec)) {
         n.code_bytes = kt * batch * M * 128;
-        n.scale_bytes = align256(kt * batch * M * 8 + 8);     // (the 256 x 256 kernel reads scales two rows at a time)
+        n.scale_bytes = align256(kt * batch * M * 8 + MXW4_SCALE_PAD);     // (the 256 x 256 kernel reads scales two rows at a time)
     }
     if (mx_skinny(M, N)) return n;
     double best = 0;
@@ -474,6 +483,8 @@ MxPlan mx_plan(int batch, int M, int N, int K, bool from_bf16, bool vec) {
         }
     }
     n.w4 = (double)((mx_tiles({256, 256, 0}, batch, M, N) + 255) / 256) * MX_W4_US < best;
+    // (scales that the caller stored end with their last row: an odd one needs MXW4_SCALE_PAD bytes behind it, so they are copied)
+    if (n.w4 && !from_bf16 && M % 2) n.scale_bytes = align256(kt * batch * M * 8 + MXW4_SCALE_PAD);
     if (n.w4) return n;
     // few tiles and a long K: split it while a split keeps 24 K tiles (6 us; joining two splits costs about 4).  (A larger tile is only
     // chosen when there are more than 256 of the next smaller one, so more than 128 of its own.)
@@ -507,7 +518,7 @@ int mx_launch(MxArgs& p, const MxPlan& n, hipStream_t st) {
         else hipLaunchKernelGGL((gemm_mxfp4_skinny_kernel<EPI, 2, false>), grid, dim3(64 * SK_WAVES), 0, st, p);
         return EA_OK;
     }
-    if (EPI != EA_EPI_F32_OUT && n.w4 && (n.scale_bytes || p.M % 2 == 0)) {
+    if (EPI != EA_EPI_F32_OUT && n.w4) {             // (its epilogue goes through bf16 images of the tile)
         const int64_t as_bytes = n.scale_bytes ? n.scale_bytes : p.a_rows * p.kt * 8;
         const int rc = ea_gemm_mxfp4_w4_launch(p.A, p.As, as_bytes, p.W, p.Ws, p.bias, p.C, p.res, p.gate, p.batch, p.M, p.N, p.kt, p.ldc, p.cbs, p.ldres,
                                                p.rbs, p.gbs, EPI, st);
@@ -592,6 +603,11 @@ extern "C" int ea_gemm_mxfp4(const uint8_t* A, const uint8_t* A_scales, const ea
         p.A = ws;
         p.As = ws + n.code_bytes;
         p.X = nullptr;
+    } else if (n.scale_bytes && epilogue != EA_EPI_F32_OUT) {      // (fp32 results do not take that kernel)
+        const int64_t words = p.a_rows * p.kt;
+        hipLaunchKernelGGL(copy_scales_kernel, dim3((unsigned)((words + 1023) / 1024)), dim3(256), 0, st, reinterpret_cast<const uint64_t*>(A_scales),
+                           reinterpret_cast<uint64_t*>(ws), words);
+        p.As = ws;
     }
     int rc;
     switch (epilogue) {

@@ -159,8 +159,8 @@ int ea_mxfp4_dequantize_bf16(const uint8_t* codes, const uint8_t* scales, ea_bf1
  * C bf16 (fp32) row stride ldc >= N, c_batch_stride >= N (batch > 1); res as ea_gemm_bf16 (may be C itself); gate fp32 [batch][gate_batch_stride].
  * N, ldc, ldres and the batch strides of C and res % 8 == 0, gate_batch_stride % 4 == 0, pointers 16-byte (scales 8-byte) aligned.
  * workspace: ea_gemm_mxfp4_workspace_bytes() bytes of the caller's (a_is_bf16 = 1 when A_bf16 is given), 0 for many shapes: stored
- * activations, and fp32 partial products of a K split, summed in a fixed order (results do not depend on timing).  Calls that may
- * run at the same time need one each. */
+ * activations, their scales (large products of an odd M), and fp32 partial products of a K split, summed in a fixed order (results do
+ * not depend on timing).  Calls that may run at the same time need one each. */
 int64_t ea_gemm_mxfp4_workspace_bytes(int batch, int M, int N, int K, int a_is_bf16);
 int ea_gemm_mxfp4(const uint8_t* A, const uint8_t* A_scales, const ea_bf16* A_bf16, const uint8_t* W, const uint8_t* W_scales,
                   const float* bias, void* C, const ea_bf16* res, const float* gate, int batch, int M, int N, int K, int64_t lda,
