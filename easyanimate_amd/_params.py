@@ -17,61 +17,66 @@ def _key(p: torch.Tensor):
     return (p.data_ptr(), p._version, p.device, p.dtype, tuple(p.shape))
 
 
-def _raw_stream(dev: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+# (called for every derived weight of a forward pass: the C functions themselves, 0.1 us each)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # of a device's index
+_stream_captures = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
-def _capturing(dev: torch.device) -> bool:
-    if torch._C._cuda_getDevice() == dev.index:
-        return torch._C._cuda_isCurrentStreamCapturing()
-    with torch.cuda.device(dev):
-        return torch._C._cuda_isCurrentStreamCapturing()
+def _capturing(index: int) -> bool:
+    if _current_device() == index:
+        return _stream_captures()
+    with torch.cuda.device(index):
+        return _stream_captures()
 
 
 _of_graphs: Dict[int, object] = {}      # copies that a captured graph reads: replays may come after the cache has let go of them
 
 
 class _Made:
-    """Where a derived copy was made: the stream, an event behind its kernels, and the streams that already stand behind that."""
-    __slots__ = ("event", "streams")
+    """Where a derived copy was made: the device, an event behind its kernels, and the streams that already stand behind that."""
+    __slots__ = ("index", "event", "streams")
 
-    def __init__(self, dev: torch.device):
+    def __init__(self, index: int):
+        self.index = index
         self.event = torch.cuda.Event()
-        self.event.record(torch.cuda.current_stream(dev))
-        self.streams = {_raw_stream(dev)}
+        self.event.record(torch.cuda.current_stream(index))
+        self.streams = {_raw_stream(index)}
 
-    def join(self, dev: torch.device, val) -> None:
-        """Before the current stream of `dev` reads the copy: it waits for it, and the copy's memory is not used again, once it is
-        dropped, before that stream is through with it."""
-        raw = _raw_stream(dev)
-        if raw in self.streams:
-            return
-        stream = torch.cuda.current_stream(dev)
+    def join(self, raw: int, val) -> None:
+        """Before another stream reads the copy: it waits for it, and the copy's memory is not used again, once it is dropped, before
+        that stream is through with it."""
+        stream = torch.cuda.current_stream(self.index)
         stream.wait_event(self.event)
         for t in (val,) if isinstance(val, torch.Tensor) else (val.codes, val.scales):
             t.record_stream(stream)
         self.streams.add(raw)
 
 
-def derived(p: torch.Tensor, tag: str, fn: Callable[[torch.Tensor], torch.Tensor]) -> torch.Tensor:
+def derived(p: torch.Tensor, tag: str, fn: Callable[[torch.Tensor], torch.Tensor], graph_own: bool = False) -> torch.Tensor:
     """fn(p), kept until p changes; usable on any stream.  Made under graph capture it belongs to the graph (its memory is filled by
     replays) and is not kept; one that is there already when a graph is captured stays for good (nothing is to be waited for there: the
-    device was idle when the capture began, and an event from outside may not enter a graph)."""
+    device was idle when the capture began, and an event from outside may not enter a graph), or is made again (graph_own)."""
     k = (id(p), tag)
     ent = _cache.get(k)
     sig = _key(p)
     if ent is not None and ent[0] == sig:
-        if ent[2] is not None:
-            if _capturing(p.device):
-                _of_graphs[id(ent[1])] = ent[1]
-            else:
-                ent[2].join(p.device, ent[1])
-        return ent[1]
+        made = ent[2]
+        if made is None:
+            return ent[1]
+        if not _capturing(made.index):
+            raw = _raw_stream(made.index)
+            if raw not in made.streams:
+                made.join(raw, ent[1])
+            return ent[1]
+        if not graph_own:
+            _of_graphs[id(ent[1])] = ent[1]
+            return ent[1]
     with torch.no_grad():
         val = fn(p.detach())
-    if p.is_cuda and _capturing(p.device):
+    if p.is_cuda and _capturing(p.device.index):
         return val
-    _cache[k] = (sig, val, _Made(p.device) if p.is_cuda else None)
+    _cache[k] = (sig, val, _Made(p.device.index) if p.is_cuda else None)
     if k not in _finalized:      # ONE finalizer per (parameter, tag) for the parameter's lifetime: every pipeline call clears the
         try:                     # cache (invalidate_weight_cache) and recomputes -- it must not also add a finalizer each time
             weakref.finalize(p, _drop, k)
@@ -169,10 +174,10 @@ def mxfp4_weight(p):
     its replays lay out the weights as they are then, in the graph's own memory."""
     from . import ops
     make = lambda t: ops.mxfp4_quantize(t.to(torch.bfloat16))
-    if not frozen() or (p.is_cuda and _capturing(p.device)):
+    if not frozen():
         with torch.no_grad():
             return make(p.detach())
-    return derived(p, "mxfp4", make)
+    return derived(p, "mxfp4", make, graph_own=True)
 
 
 def kblocked_weight(p):

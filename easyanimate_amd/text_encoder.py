@@ -103,9 +103,8 @@ class Qwen2VLTextEncoderHIP(nn.Module):
     def _gate_ones(self) -> torch.Tensor:
         return derived(self._text[0].norm.weight, "ones", lambda t: torch.ones(self.hidden, dtype=torch.float32, device=t.device))
 
-    def _layer_mxfp4(self, layer, h, B, S, cos, sin, valid):
+    def _layer_mxfp4(self, layer, h, B, S, cos, sin, valid, ones):
         att, mlp, D, Hq, Hkv = layer.self_attn, layer.mlp, self.head_dim, self.q_heads, self.kv_heads
-        ones = self._gate_ones()
         fb = lambda lin: f32(lin.bias) if lin.bias is not None else None
         lin = lambda a, l: ops.gemm_mxfp4(a, mxfp4_weight(l.weight), fb(l))
         add = lambda a, l, res: ops.gemm_mxfp4(a, mxfp4_weight(l.weight), fb(l), ops.EPI_BIAS_GATE_RES, res=res, gate=ones)
@@ -158,10 +157,11 @@ class Qwen2VLTextEncoderHIP(nn.Module):
         four = self.weights == "mxfp4"
         vt = None if four else torch.zeros(B, Hkv, D, s_pad, dtype=torch.bfloat16, device=dev)
         h = x.reshape(B * S, d).contiguous()
+        ones = self._gate_ones()
         hidden_states = [x]
         for layer in text.layers:
             if four:
-                h = self._layer_mxfp4(layer, h, B, S, cos, sin, valid)
+                h = self._layer_mxfp4(layer, h, B, S, cos, sin, valid, ones)
                 hidden_states.append(h.view(B, S, d))
                 continue
             att, mlp = layer.self_attn, layer.mlp
@@ -174,12 +174,12 @@ class Qwen2VLTextEncoderHIP(nn.Module):
             vt[..., :S] = v.view(B, S, Hkv, D).permute(0, 2, 3, 1)            # V^T (columns >= S stay zero)
             a = ops.attention_causal_gqa(qh, kh, vt, S, D ** -0.5, valid)
             ob = f32(att.o_proj.bias) if att.o_proj.bias is not None else None
-            h = ops.gemm(a.view(B * S, Hq * D), gemm_weight(att.o_proj.weight), ob, ops.EPI_BIAS_GATE_RES, res=h, gate=self._gate_ones())
+            h = ops.gemm(a.view(B * S, Hq * D), gemm_weight(att.o_proj.weight), ob, ops.EPI_BIAS_GATE_RES, res=h, gate=ones)
             n2 = ops.rmsnorm(h, f32(layer.post_attention_layernorm.weight), self.eps)
             g = ops.gemm(n2, gemm_weight(mlp.gate_proj.weight), None)
             u = ops.gemm(n2, gemm_weight(mlp.up_proj.weight), None)
             act = ops.silu_mul(g, u)
-            h = ops.gemm(act, gemm_weight(mlp.down_proj.weight), None, ops.EPI_BIAS_GATE_RES, res=h, gate=self._gate_ones())
+            h = ops.gemm(act, gemm_weight(mlp.down_proj.weight), None, ops.EPI_BIAS_GATE_RES, res=h, gate=ones)
             hidden_states.append(h.view(B, S, d))
         last = ops.rmsnorm(h, f32(text.norm.weight), self.eps).view(B, S, d)
         # transformers: hidden_states = (embeddings, layer 1 .. layer L-1 outputs, NORMED layer L output)

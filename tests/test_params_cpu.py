@@ -36,8 +36,8 @@ class Gpu:
         def stream(dev):
             i = gpu.now
             return types.SimpleNamespace(id=i, wait_event=lambda e: gpu.log.append(("wait", i)))
-        monkeypatch.setattr(_params, "_raw_stream", lambda dev: gpu.now)
-        monkeypatch.setattr(_params, "_capturing", lambda dev: gpu.capture)
+        monkeypatch.setattr(_params, "_raw_stream", lambda index: gpu.now)
+        monkeypatch.setattr(_params, "_capturing", lambda index: gpu.capture)
         monkeypatch.setattr(torch.cuda, "Event", Event)
         monkeypatch.setattr(torch.cuda, "current_stream", stream)
         monkeypatch.setattr(_params, "_cache", {})
