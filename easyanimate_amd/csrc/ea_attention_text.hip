@@ -14,8 +14,10 @@
 // and, because K rows are fed in the order 8 (r / 4) + 4 kt + r % 4, eight consecutive keys of a 32-key block = its slice of the P^T
 // operand.  V stays row-major in memory and LDS; its transposed fragments come from ds_read_b64_tr_b16.  One pass with a running
 // maximum that is only moved when a score exceeds it by 2^8 (P then stays below 256 -- bf16 has fp32's exponent range -- and the
-// accumulators are hardly ever rescaled); P is rounded to bf16 for its product (a relative half step of 2^-8 each); the row sums are
-// those of the rounded weights, by one more product with ones, in fp32.
+// accumulators are hardly ever rescaled).  P is rounded to bf16 for its product (a relative half step of 2^-8 each): the bf16 matrix
+// instructions take no more, and a second product for what the rounding cuts off would double the work of P.V.  The results' distance
+// from 64 bits grows by it from 1.7e-3 (their own rounding) to 1.8 .. 2.4e-3, relative.  The row sums are those of the rounded weights,
+// by one more product with ones, in fp32.
 //
 //   attention_text_kernel       128 or 64 rows per workgroup (four waves, 32 or 16 rows each), K / V tiles of 64 keys double-buffered in LDS by
 //                               LDS-DMA; tiles that no row of the workgroup sees are skipped (64 at a time for documents)
@@ -511,11 +513,13 @@ __device__ __forceinline__ void store_rows(const TextArgs& p, Rows<D, RT>& R, in
 // ---- 128 or 64 rows per workgroup --------------------------------------------------------------------------------------------------
 // Bound by issue slots, not by memory or the matrix pipe: for one wave of 32 rows and a 32-key block at D = 128 the matrix instructions
 // take 544 clocks of about 1240, the softmax 98 vector and 74 scalar instructions; two waves of a SIMD cover each other in part (matrix
-// pipe busy 44 %).  1000 TFLOP/s at 28 / 4 heads, 8192 tokens, D = 128; 851 at 32 / 32 heads, 4096 tokens (323 us; cap 365 us, bias
-// 351 us); 790 at D = 64 (2 x 32 heads, 4096 tokens: 350 us).  At D = 64 the registers of three workgroups per CU are given room for:
-// 480 against 554 us with a cap, 448 against 533 us with a bias, 621 against 724 us with both (which costs 20 bytes of scratch).  Measured
-// and not taken: a tile's two blocks overlapped inside a wave of 32 rows (spills at D = 128, 407 against 364 us at D = 64; waves of 16
-// rows have the room), K fragments read a block ahead, and requests spread between the instructions (343 against 333 us).
+// pipe busy 44 %).  974 TFLOP/s at 28 / 4 heads, 8192 tokens, D = 128 (988 us); 844 at 32 / 32 heads, 4096 tokens (326 us; cap 369 us,
+// bias 324 us); 785 at D = 64 (2 x 32 heads, 4096 tokens: 350 us), where ea_attention_fwd_bf16's loop reaches 1288 on long sequences: it
+// overlaps blocks inside a wave and keeps no maximum per block, this one overlaps waves only.  At D = 64 the registers of three workgroups
+// per CU are given room for: 485 against 554 us with a cap, 424 against 533 us with a bias, 621 against 724 us with both (which costs 20
+// bytes of scratch).  Measured and not taken in this loop: a tile's two blocks overlapped inside a wave of 32 rows (spills at D = 128, 407
+// against 364 us at D = 64; waves of 16 rows have the room), K fragments read a block ahead, and requests spread between the
+// instructions (343 against 333 us).
 constexpr int TKEYS = 64;
 // floats per head of a tile's bias window: its 64 keys against every query of the row tile
 __host__ __device__ __forceinline__ int bias_window(int trows, int pack) { return TKEYS + (trows - 1) / pack + 2; }

@@ -434,7 +434,9 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_join_kernel(MxArgs p) {
     mx_store4<EPI>(p, b, m, n0, v, mx_bias(p, n0), mx_gate<EPI>(p, b, n0), mx_res<EPI>(p, b, m, n0));
 }
 
-// a K tile's scales of a row are 8 bytes: stored scales, copied to where the 256 x 256 kernel may read behind the last row
+// a K tile's scales of a row are 8 bytes: stored scales, copied to where the 256 x 256 kernel may read behind the last row (one more
+// launch, 3 us; 8191 x 8192 x 8192 226 us, 287 on 256 x 128 tiles, which need no copy; 3999 x 8200 x 3584 102 and 97: bits that do not
+// depend on how the activations came are worth that)
 __global__ __launch_bounds__(256) void copy_scales_kernel(const uint64_t* __restrict__ from, uint64_t* __restrict__ to, int64_t words) {
     const int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x;
 #pragma unroll

@@ -142,9 +142,9 @@ __global__ __launch_bounds__(256) void gn_apply_kernel(const unsigned short* __r
 // per thread (16 registers) and an element costs one fma (+ 4 ops of SiLU as x * rcp(1 + 2^(-x log2 e))); no integer
 // division in the loop.  HBM-bound (4 B per element).
 // Round 5: the activation is a template parameter (the run-time `act` cost a select per element and the SiLU arithmetic on layers
-// that have none) and the arithmetic is packed fp32 on channel pairs (v_pk_fma / v_pk_mul / v_pk_add: the same IEEE operations per
-// element, bit-identical): 353 -> ~210 instructions per 32 elements.  That alone changed nothing (the kernel runs as fast without
-// SiLU as with it); what did is the order in which it walks memory, see the loop.
+// that have none) and the arithmetic is written on channel pairs (the library is built without the packed fp32 instructions, so a pair
+// is two plain ones).  The arithmetic is not what bounds it (it runs as fast without SiLU as with it): the order in which it walks
+// memory is, see the loop.
 typedef float gn_f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 gn_bf16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned gn_u32x4 __attribute__((ext_vector_type(4)));

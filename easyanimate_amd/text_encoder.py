@@ -19,7 +19,10 @@ Text-only: image / video inputs are refused (the EasyAnimate pipelines never pas
 
 `weights="mxfp4"` runs the same layers with 4-bit Linear layers (ops.gemm_mxfp4: weights and activations in blocks of 32 e2m1 codes
 under one power-of-two scale; a layer's q / k / v and gate / up products share one quantised input) and ops.attention_text, which reads
-V as the projection left it: a fast approximation, 0.1 to 0.2 relative error per product.  The default is the bf16 path above."""
+V as the projection left it.  A coarse approximation: 0.16 relative error (L2) per product on normal inputs, 0.20 where one channel in 256
+is 20 times the others.  On random-init weights of the 7B widths, where nothing damps it, `hidden_states[-2]` is 0.75 away from the bf16
+path's after 4 layers and 1.2, unrelated, after 28; no checkpoint was at hand to say what trained weights do.  The 4-bit copies stand
+beside the model's own weights.  The default is the bf16 path above."""
 from __future__ import annotations
 
 import types
