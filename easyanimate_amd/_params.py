@@ -30,7 +30,9 @@ def _capturing(index: int) -> bool:
         return _stream_captures()
 
 
-_of_graphs: Dict[int, object] = {}      # copies that a captured graph reads: replays may come after the cache has let go of them
+# copies that a captured graph reads, by key: replays may come after the cache has let go of them.  They go with their parameter (whose own
+# memory the graph reads too); a program that captures again after every invalidate_weight_cache() keeps a set of copies for each graph
+_of_graphs: Dict[Tuple[int, str], dict] = {}
 
 
 class _Made:
@@ -70,7 +72,7 @@ def derived(p: torch.Tensor, tag: str, fn: Callable[[torch.Tensor], torch.Tensor
                 made.join(raw, ent[1])
             return ent[1]
         if not graph_own:
-            _of_graphs[id(ent[1])] = ent[1]
+            _of_graphs.setdefault(k, {})[id(ent[1])] = ent[1]
             return ent[1]
     with torch.no_grad():
         val = fn(p.detach())
@@ -88,6 +90,7 @@ def derived(p: torch.Tensor, tag: str, fn: Callable[[torch.Tensor], torch.Tensor
 
 def _drop(k) -> None:
     _cache.pop(k, None)
+    _of_graphs.pop(k, None)
     _finalized.discard(k)
 
 

@@ -1,5 +1,6 @@
 """The cache of derived weights: streams, graph capture and regions of frozen weights, on the CPU with stand-ins for streams and
 events (the order of the calls is what counts)."""
+import gc
 import types
 
 import pytest
@@ -137,5 +138,9 @@ def test_what_a_graph_reads_outlives_the_cache(gpu):
         assert _params.derived(w, "f32", gpu.make) is one
     gpu.capture = False
     _params.invalidate_weight_cache()
-    assert list(_params._of_graphs.values()) == [one]
+    kept = lambda: [v for d in _params._of_graphs.values() for v in d.values()]
+    assert kept() == [one]
     assert _params.derived(w, "f32", gpu.make) is not one                   # eager calls make theirs anew
+    del w                                                                   # the parameter goes, and with it what its graphs could read
+    gc.collect()
+    assert kept() == []
