@@ -587,6 +587,7 @@ extern "C" int ea_gemm_mxfp4(const uint8_t* A, const uint8_t* A_scales, const ea
     if (epilogue == EA_EPI_BIAS_GATE_RES)
         EA_REQUIRE(res && gate && ldres % 8 == 0 && res_batch_stride % 8 == 0 && gate_batch_stride % 4 == 0 && ((uintptr_t)res | (uintptr_t)gate) % 16 == 0,
                    "ea_gemm_mxfp4: gated-residual epilogue needs aligned res and gate");
+    EA_REQUIRE(C != (const void*)A && C != (const void*)A_bf16 && C != (const void*)W, "ea_gemm_mxfp4: C must not overlap the activations or the weight");
     const MxPlan n = mx_plan(batch, M, N, K, A_bf16 != nullptr, A_bf16 && mx_vec(A_bf16, K, lda, a_batch_stride));
     const int64_t need = n.code_bytes + n.scale_bytes + n.part_bytes;
     EA_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),

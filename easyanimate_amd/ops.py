@@ -326,8 +326,8 @@ def mxfp4_dequantize(q: Mxfp4) -> torch.Tensor:
 def gemm_mxfp4(A: Union[torch.Tensor, Mxfp4], W: Mxfp4, bias: Optional[torch.Tensor], epilogue: int = EPI_BIAS,
                out: Optional[torch.Tensor] = None, res: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[b] = epi(A[b] @ W.T + bias) over 4-bit operands, W of a [N, K] nn.Linear weight (N % 8 == 0).  A: bf16 [B, M, K] or [M, K]
-    (quantised here: mxfp4_quantize's values), or the Mxfp4 of [M, K].  bias fp32 [N]; out bf16 [B, M, N] (fp32 for EPI_F32_OUT); res
-    bf16 like out (may alias out); gate fp32 [B, N] ([N] for two-dimensional A); epilogues as gemm()."""
+    (quantised here: mxfp4_quantize's values), or the Mxfp4 of [M, K].  bias fp32 [N]; out bf16 [B, M, N] (fp32 for EPI_F32_OUT), not
+    overlapping A or W; res bf16 like out (may alias out); gate fp32 [B, N] ([N] for two-dimensional A); epilogues as gemm()."""
     if not isinstance(W, Mxfp4):
         raise TypeError(f"W: expected Mxfp4, got {type(W).__name__}")
     N, K = W.rows, W.k

@@ -156,7 +156,8 @@ int ea_mxfp4_dequantize_bf16(const uint8_t* codes, const uint8_t* scales, ea_bf1
  * ea_gemm_bf16 (EA_EPI_F32_OUT: C, ldc and c_batch_stride in floats).  W: codes / scales of [N, K].  The activations are either
  *   A / A_scales of [batch * M, K] (element b = rows [b M, (b + 1) M)), A_bf16 NULL, or
  *   A_bf16 [batch][M][lda] (any strides), A and A_scales NULL: quantised on the way or into the workspace -- same codes, same result.
- * C bf16 (fp32) row stride ldc >= N, c_batch_stride >= N (batch > 1); res as ea_gemm_bf16 (may be C itself); gate fp32 [batch][gate_batch_stride].
+ * C bf16 (fp32) row stride ldc >= N, c_batch_stride >= N (batch > 1), overlapping neither the activations nor the weight; res as
+ * ea_gemm_bf16 (may be C itself); gate fp32 [batch][gate_batch_stride].
  * N, ldc, ldres and the batch strides of C and res % 8 == 0, gate_batch_stride % 4 == 0, pointers 16-byte (scales 8-byte) aligned.
  * workspace: ea_gemm_mxfp4_workspace_bytes() bytes of the caller's (a_is_bf16 = 1 when A_bf16 is given), 0 for many shapes: stored
  * activations, their scales (large products of an odd M), and fp32 partial products of a K split, summed in a fixed order (results do
