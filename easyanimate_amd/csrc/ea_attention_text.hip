@@ -1024,6 +1024,7 @@ extern "C" int ea_attention_text_bf16(const ea_bf16* q, const ea_bf16* k, const 
     EA_REQUIRE(kv_len > 0, "ea_attention_text_bf16: no keys");
     EA_REQUIRE(q && k && v && out && strides, "ea_attention_text_bf16: null tensor");
     EA_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15) == 0, "ea_attention_text_bf16: 16-byte alignment");
+    EA_REQUIRE(out != q && out != k && out != v, "ea_attention_text_bf16: out must not overlap q, k or v");
     for (int i = 0; i < 11; ++i)
         EA_REQUIRE(strides[i] % 8 == 0 && strides[i] >= 0, "ea_attention_text_bf16: strides must be non-negative multiples of 8 elements");
     EA_REQUIRE((batch == 1 || strides[9] >= (int64_t)q_heads * head_dim) && (q_len == 1 || strides[10] >= (int64_t)q_heads * head_dim),
